@@ -47,6 +47,7 @@ FACK_W_PACKED = 1
 
 FACK_DTYPE_F32 = 0
 FACK_DTYPE_BF16 = 1
+FACK_DTYPE_F16 = 2
 
 FACK_GEMM_BF16 = 0
 FACK_GEMM_I8 = 1
@@ -73,6 +74,15 @@ SIGNATURES = {
                                       _c_int, _c_int, _c_int, _c_int, _c_p]),
     "fack_gather_interleave": (_c_int, [_c_p, _c_int, _c_int, _c_int, _c_p, _c_i64, _c_p]),
     "fack_quant_act": (_c_int, [_c_p, _c_int, _c_i64, _c_int, _c_int, _c_p, _c_i64, _c_p, _c_i64, _c_i64, _c_p]),
+    "fack_moe_sort_workspace_size": (_c_int, [_c_int] * 3 + [ctypes.POINTER(_c_sz)]),
+    "fack_moe_sort": (_c_int, [_c_p, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p, _c_p, _c_p, _c_sz, _c_p]),
+    "fack_moe_gather": (_c_int, [_c_p, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_p, _c_p, _c_int, _c_p, _c_i64,
+                                 _c_p]),
+    "fack_moe_gather_quant": (_c_int, [_c_p, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_p, _c_p, _c_int, _c_p, _c_i64,
+                                       _c_p, _c_i64, _c_p]),
+    "fack_moe_combine": (_c_int, [_c_p, _c_int, _c_i64, _c_p, _c_int, _c_int, _c_int, _c_p, _c_p, _c_i64, _c_p]),
+    "fack_moe_combine_bwd": (_c_int, [_c_p, _c_int, _c_i64, _c_p, _c_i64, _c_p, _c_int, _c_int, _c_int, _c_p, _c_p,
+                                      _c_int, _c_p, _c_i64, _c_p, _c_p]),
     "fack_device_status": (_c_int, [_c_p, ctypes.POINTER(ctypes.c_uint), _c_int]),
     "fack_gemm_tn_plan": (_c_int, [_c_int] * 7 + [ctypes.POINTER(_c_int)] * 3),
     "fack_gemm_tn": (_c_int, [_c_int, _c_p, _c_i64, _c_p, _c_int, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_i64,

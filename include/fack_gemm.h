@@ -63,10 +63,12 @@ enum fack_gemm_kind {
   FACK_GEMM_I8 = 1       /* int8 A, B; s32 accumulation, per-row/column scales  */
 };
 
-/* Element types of the activation input to fack_quant_act (argument `x_dtype`). */
+/* Element types: of the activation input to fack_quant_act (argument
+ * `x_dtype`; F32 and BF16), and of the fack_moe_* and fack_gemv_w4 operands. */
 enum fack_dtype {
   FACK_DTYPE_F32 = 0,    /* fp32                                               */
-  FACK_DTYPE_BF16 = 1    /* bf16                                               */
+  FACK_DTYPE_BF16 = 1,   /* bf16                                               */
+  FACK_DTYPE_F16 = 2     /* fp16                                               */
 };
 
 /* Status and version helpers: no counterpart in the reference, whose errors
@@ -447,6 +449,57 @@ int fack_gemm_tn_plan(int kind, int M, int N, int K, int tile_m_request, int til
 int fack_gemm_tn(int kind, const void* a, int64_t lda, const void* b, int b_packed, int64_t ldb,
                  const float* a_scale, const float* b_scale, const float* bias, void* out, int64_t ldo, int M,
                  int N, int K, int tile_m, int tile_n, int split_k, void* stream);
+
+/*
+ * Tokens sorted by expert and back: the data movement around the expert
+ * products of a routed layer.  No counterpart in the reference.
+ *
+ * The plan of T tokens with topk expert ids each (row-major int32 or int64
+ * ids [T, topk]; ids_bytes = 4 or 8):
+ *   offsets[e]  (E + 1 entries) = pairs p = t*topk + j with 0 <= ids[p] < e;
+ *   row_of[p]   = offsets[e] + the pairs of the same expert before p: the
+ *                 pair's sorted row (stable), or -1 when ids[p] is outside
+ *                 [0, E) (an expert of another rank);
+ *   src[r]      = p, the inverse; -1 for the rows behind offsets[E].
+ * 1 <= E <= 1024, 1 <= topk <= 64, T*topk < 2^31.  The workspace (0 bytes for
+ * few pairs) is overwritten by each call: calls that may overlap need one each.
+ *
+ * The others read row_of and offsets of such a plan (an entry outside the
+ * rows counts as -1), take row strides in elements (0 for a broadcast input
+ * row) and run on FACK_DTYPE_F32, _BF16 or _F16 rows of D elements,
+ * 1 <= D <= 2^20, in any alignment of the element type; rows that allow 16-byte
+ * accesses (base, stride and D) go faster.  Sorted buffers hold T*topk rows; rows
+ * without a pair are written as zeros (their scales as 1).
+ *
+ *   fack_moe_gather        y[row_of[t, j]] = x[t]
+ *   fack_moe_gather_quant  xq, x_scale of row row_of[t, j] = the e4m3 codes and
+ *                          per-128 scales of x[t] (fp32 or bf16; K % 128 == 0,
+ *                          16-byte aligned rows): scale = amax/240, 1 where that
+ *                          is 0, codes e4m3fn(clamp(x/scale, -240, 240)), the
+ *                          values of fack_quant_act; a group that holds NaN
+ *                          gets scale and codes NaN
+ *   fack_moe_combine       out[t] = sum_j weights[t, j] * y[row_of[t, j]] over the
+ *                          pairs with a row, in fp32 in the order of j, rounded
+ *                          once; weights fp32 [T, topk] contiguous, NULL for
+ *                          ones (then it is the backward of fack_moe_gather)
+ *   fack_moe_combine_bwd   dy[row_of[t, j]] = weights[t, j] * dout[t] (dy NULL:
+ *                          not wanted) and dweights[t, j] = <dout[t],
+ *                          y[row_of[t, j]]> in fp32, 0 without a row (dweights
+ *                          NULL: not wanted, y is then unused)
+ */
+int fack_moe_sort_workspace_size(int T, int topk, int num_experts, size_t* bytes);
+int fack_moe_sort(const void* ids, int ids_bytes, int T, int topk, int num_experts, int32_t* row_of, int32_t* src,
+                  int32_t* offsets, void* workspace, size_t workspace_bytes, void* stream);
+int fack_moe_gather(const void* x, int dtype, int64_t ldx, int T, int topk, int D, const int32_t* row_of,
+                    const int32_t* offsets, int num_experts, void* y, int64_t ldy, void* stream);
+int fack_moe_gather_quant(const void* x, int dtype, int64_t ldx, int T, int topk, int K, const int32_t* row_of,
+                          const int32_t* offsets, int num_experts, void* xq, int64_t ldq, float* x_scale, int64_t lds,
+                          void* stream);
+int fack_moe_combine(const void* y, int dtype, int64_t ldy, const float* weights, int T, int topk, int D,
+                     const int32_t* row_of, void* out, int64_t ldo, void* stream);
+int fack_moe_combine_bwd(const void* dout, int dtype, int64_t ldd, const void* y, int64_t ldy, const float* weights, int T,
+                         int topk, int D, const int32_t* row_of, const int32_t* offsets, int num_experts, void* dy,
+                         int64_t lddy, float* dweights, void* stream);
 
 /*
  * Reads (and with reset != 0 clears) the current device's error word, which a
