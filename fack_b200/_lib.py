@@ -83,6 +83,10 @@ SIGNATURES = {
     "fack_moe_combine": (_c_int, [_c_p, _c_int, _c_i64, _c_p, _c_int, _c_int, _c_int, _c_p, _c_p, _c_i64, _c_p]),
     "fack_moe_combine_bwd": (_c_int, [_c_p, _c_int, _c_i64, _c_p, _c_i64, _c_p, _c_int, _c_int, _c_int, _c_p, _c_p,
                                       _c_int, _c_p, _c_i64, _c_p, _c_p]),
+    "fack_gemv_w4": (_c_int, [_c_p, _c_int, _c_i64, _c_p, _c_p, _c_int, _c_p, _c_int, _c_p, _c_i64, _c_int, _c_int,
+                              _c_int, _c_p]),
+    "fack_gemv_w4_experts": (_c_int, [_c_p, _c_int, _c_i64, _c_p, _c_p, _c_int, _c_p, _c_int, _c_p, _c_p, _c_int,
+                                      _c_int, _c_int, _c_p, _c_i64, _c_int, _c_int, _c_p]),
     "fack_device_status": (_c_int, [_c_p, ctypes.POINTER(ctypes.c_uint), _c_int]),
     "fack_gemm_tn_plan": (_c_int, [_c_int] * 7 + [ctypes.POINTER(_c_int)] * 3),
     "fack_gemm_tn": (_c_int, [_c_int, _c_p, _c_i64, _c_p, _c_int, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_i64,

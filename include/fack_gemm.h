@@ -502,6 +502,35 @@ int fack_moe_combine_bwd(const void* dout, int dtype, int64_t ldd, const void* y
                          int64_t lddy, float* dweights, void* stream);
 
 /*
+ * Products of a few tokens with 4-bit weights.  No counterpart in the reference.
+ *
+ *   y[m, n] = sum_k x[m, k] * (c[n, k] - z[k/G, n]) * s[k/G, n]
+ *
+ * x [M, K] and y [M, N] are FACK_DTYPE_BF16 or _F16 with row strides ldx, ldy in
+ * elements (x rows 16-byte aligned: ldx % 8 == 0, or 0 for one row for all);
+ * w [N, K/2] holds two codes 0..15 a byte, even k in the low nibble; scales
+ * [K/G, N] are fp32 (scale_dtype FACK_DTYPE_F32) or of x's type; zeros
+ * [K/G, N] are bytes 0..15 (the low four bits are read), NULL for 8 everywhere.
+ * w, scales and zeros are contiguous and 16-byte aligned.  N % 16 == 0;
+ * G = 32, 64 or a multiple of 128; K % G == 0, K <= 2^20; M >= 1 (meant for M
+ * up to about 32: more tokens are taken 8 or 16 at a time).  Products are exact, sums
+ * fp32, one rounding to y's type; the same call gives the same bits.
+ * Capturable; allocates nothing.
+ *
+ * fack_gemv_w4_experts: y [T*topk, N] from the weights of each sorted row's
+ * expert: w [E, N, K/2], scales and zeros [E, K/G, N], offsets (and src) of a
+ * fack_moe_sort plan.  With src, x is [T, K] and row r of y takes x's row
+ * src[r] / topk (a src outside the pairs: a row of zeros); with src NULL, x is
+ * [T*topk, K], sorted.  Rows behind offsets[E] are written as zeros (all rows,
+ * where offsets do not ascend within 0..T*topk).
+ */
+int fack_gemv_w4(const void* x, int dtype, int64_t ldx, const void* w, const void* scales, int scale_dtype,
+                 const void* zeros, int group, void* y, int64_t ldy, int M, int N, int K, void* stream);
+int fack_gemv_w4_experts(const void* x, int dtype, int64_t ldx, const void* w, const void* scales, int scale_dtype,
+                         const void* zeros, int group, const int32_t* src, const int32_t* offsets, int T, int topk,
+                         int num_experts, void* y, int64_t ldy, int N, int K, void* stream);
+
+/*
  * Reads (and with reset != 0 clears) the current device's error word, which a
  * kernel sets when a bounded wait inside it gives up.  Synchronises `stream`.
  * *flags == 0 means no kernel has reported a problem.  Returns
