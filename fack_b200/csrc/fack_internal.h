@@ -22,6 +22,12 @@ int sm100_device(int* sms);
 int encode_bytes_2d(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t outer, uint64_t row_bytes,
                     uint32_t box_inner, uint32_t box_outer, bool swizzle128);
 
+// 2-D tensor map over elements of 1, 2 or 4 bytes: `outer` rows of `inner`
+// elements, rows `row_bytes` apart, 64-byte swizzle or none; out-of-range
+// elements read as zeros.  FACK_ERR_BAD_ALIGN if the driver refuses the layout.
+int encode_elems_2d(CUtensorMap* map, const void* ptr, int elem_bytes, uint64_t inner, uint64_t outer, uint64_t row_bytes,
+                    uint32_t box_inner, uint32_t box_outer, bool swizzle64);
+
 // Device address of the library's status word on the current device (NULL
 // on failure); kernels OR a flag into it when a bounded wait gives up.
 unsigned int* device_status_word();

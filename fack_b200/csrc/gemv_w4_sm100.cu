@@ -29,6 +29,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include <mutex>
@@ -41,11 +42,13 @@ namespace fack_w4 {
 
 using namespace fack;
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
-constexpr int kBlkK = 128;                     // k per stage
+constexpr int kWarps = 8;                      // that multiply; one more brings the data
+constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kBlkK = 128;                     // k per warp and stage
+constexpr int kMaxStages = 8;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopk = 64;
+constexpr unsigned kStW4 = 128u;               // status flag: a wait in these kernels gave up
 
 struct Args {
   const void* x;                               // [rows or tokens, K]
@@ -59,7 +62,11 @@ struct Args {
   const int* offsets;                          // [E + 1], NULL: one weight, all rows
   int rows, topk, N, K, G, E;
   int tile;                                    // tokens per tile (<= 8 NT)
+  int split;                                   // slices of K among a CTA's warps: 1, 2, 4 or 8
+  int stages;
   int scale_f32;
+  unsigned int* status;
+  uint64_t timeout_ns;
 };
 
 // A word's codes 0..7 as four registers of two 16-bit floats each, (c - z) *
@@ -109,33 +116,43 @@ __device__ __forceinline__ void unpack_codes(uint32_t w, uint32_t minus_z, uint3
   h[3] = fma2<T>(v & 0x00f000f0u, Codes<T>::kHigh, minus_z);
 }
 
+// d = a * b + c on the warp's 16 x 8 tile
+#define FACK_W4_MMA(TYPE)                                                                                              \
+  asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE                                                           \
+      ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"                                       \
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])                                                                 \
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]))
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1, __nv_bfloat16*) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                                         uint32_t b1, const float (&c)[4], __nv_bfloat16*) {
+  FACK_W4_MMA("bf16");
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1, __half*) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                                         uint32_t b1, const float (&c)[4], __half*) {
+  FACK_W4_MMA("f16");
 }
-
+#undef FACK_W4_MMA
 // d (+)= a * b: the first product of a group starts from zero
 template <typename T>
 __device__ __forceinline__ void mma_step(float (&d)[4], bool first, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-  if (first) d[0] = d[1] = d[2] = d[3] = 0.0f;
-  mma16816(d, a0, a1, a2, a3, b0, b1, static_cast<T*>(nullptr));
+  const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (first)
+    mma16816(d, a0, a1, a2, a3, b0, b1, zero, static_cast<T*>(nullptr));
+  else
+    mma16816(d, a0, a1, a2, a3, b0, b1, d, static_cast<T*>(nullptr));
 }
 
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
   return v;
+}
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[1]) { v[0] = lds32(a); }
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[2]) {
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a));
+}
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[4]) {
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a));
 }
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
@@ -157,55 +174,91 @@ __device__ __forceinline__ float scale_of(uint32_t bits, __half*) {
   return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
 }
 
-// One warp's stage of the ring: 16R weight rows of 64 bytes (16-byte chunk c of
-// row r at c ^ (r/2 & 3): the reads of a word per row and quad lane have no bank
-// conflict), the tokens' rows of 256 bytes (chunk c of token m at c ^ 4(m & 1)),
-// the groups' scales and zero points of the 16R rows.  A multiple of 256 bytes, so
-// that the exclusive-or can be done on addresses.
+// A CTA's item is 16R * share output rows (share = 8 / split) and a tile of
+// tokens; a stage of its ring holds `split` consecutive K blocks of them, one for
+// each slice.  Warp (part, slice) multiplies rows 16R * part .. of block `slice`.
+//   weights: per slice, rows of 64 bytes in the 64-byte swizzle (16-byte chunk c of
+//     row r at c ^ (r/2 & 3));
+//   tokens: rows of split * 256 bytes and a pad;
+//   scales and zero points: per box of at most 256 output rows, a row for each
+//     group of the stage's blocks.
+// How the chunks are read: a step j of the MMA takes 8 consecutive codes (one
+// word) a lane and row.  With groups of 64 or 128 k a lane's two words may be
+// consecutive, one 8-byte read (WV = 2), else one (WV = 1), since a step may not mix
+// groups: step j of quad lane q is word WV q + j % WV of part j / WV.  The pads put
+// the tokens' reads on different banks.
 template <int R, int FL>
 struct Stage {
   static constexpr int kGroups = kBlkK / FL;
   static constexpr int kRows = 16 * R;
-  static constexpr int kTokenAt = kRows * 64;
-  __host__ __device__ static int scale_at(int tile) { return kTokenAt + tile * 256; }
-  __host__ __device__ static int zero_at(int tile, int es) { return scale_at(tile) + kGroups * kRows * es; }
-  __host__ __device__ static int bytes(int tile, int es, bool zeros) {
-    return (zero_at(tile, es) + (zeros ? kGroups * kRows : 0) + 255) / 256 * 256;
+  static constexpr int kWords = FL == 32 || R == 4 ? 1 : 2;   // WV (R = 4 has no registers for more)
+  static constexpr int kWeightBytes = kWarps * kRows * 64;
+  static constexpr int kPad = kWords == 1 ? 64 : 16;
+  __host__ __device__ static int up(int v, int to) { return (v + to - 1) / to * to; }
+  __host__ __device__ static int box_rows(int split) { return kRows * (kWarps / split) < 256 ? kRows * (kWarps / split) : 256; }
+  __host__ __device__ static int boxes(int split) { return kRows * (kWarps / split) / box_rows(split); }
+  __host__ __device__ static int x_pitch(int split) { return split * 256 + kPad; }
+  __host__ __device__ static int scale_at(int tile, int split) { return up(kWeightBytes + tile * x_pitch(split), 128); }
+  __host__ __device__ static int scale_box(int split, int es) { return up(split * kGroups * box_rows(split) * es, 128); }
+  __host__ __device__ static int zero_at(int tile, int split, int es) {
+    return scale_at(tile, split) + boxes(split) * scale_box(split, es);
+  }
+  __host__ __device__ static int zero_box(int split) { return up(split * kGroups * box_rows(split), 128); }
+  __host__ __device__ static int bytes(int tile, int split, int es, bool zeros) {
+    return up(zero_at(tile, split, es) + (zeros ? boxes(split) * zero_box(split) : 0), 1024);
   }
 };
 template <int R, int NT>
 struct Sums {                                  // the warps' partial sums
   static constexpr int kPitch = 8 * NT + 1;
-  static constexpr int kBytes = kWarps * 16 * R * kPitch * 4;
+  static int bytes(int split) { return split > 1 ? kWarps * 16 * R * kPitch * 4 : 0; }
 };
 
 struct Item {
   int expert, n0, row0, count;
 };
 
-template <typename T, int R, int NT, int FL, bool ZP, int STAGES>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) gemv_w4_kernel(const __grid_constant__ Args p) {
+template <typename T, int R, int NT, int FL, bool ZP>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
+    gemv_w4_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap s_map,
+                   const __grid_constant__ CUtensorMap z_map, const __grid_constant__ Args p) {
   using S = Stage<R, FL>;
   using C = Codes<T>;
   constexpr int kRows = S::kRows, kPitch = Sums<R, NT>::kPitch;
-  extern __shared__ __align__(256) uint8_t smem[];
-  __shared__ int part[2][kWarps];
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ int part[2][kWarps + 1];
+  __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages];
+  __shared__ int abort_flag_s, routed_s;         // rows of an expert: the rest are zeros
+  volatile int* abort_flag = &abort_flag_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int split = p.split, share = kWarps / split, item_rows = kRows * share;
   const int es = p.scale_f32 ? 4 : 2;
-  const int stage_bytes = S::bytes(p.tile, es, ZP);
-  const uint32_t ring = smem_addr(smem) + warp * (STAGES * stage_bytes);
-  float* red = reinterpret_cast<float*>(smem + kWarps * STAGES * stage_bytes);
+  const int box_rows = S::box_rows(split), boxes = S::boxes(split), x_pitch = S::x_pitch(split);
+  const int stage_bytes = S::bytes(p.tile, split, es, ZP);
+  const int scale_at = S::scale_at(p.tile, split), scale_box = S::scale_box(split, es);
+  const int zero_at = S::zero_at(p.tile, split, es), zero_box = S::zero_box(split);
+  const uint32_t ring = smem_addr(smem);
+  float* red = reinterpret_cast<float*>(smem + p.stages * stage_bytes);
   // the experts that have rows: number, first and last sorted row, running count of token tiles
   const int room = p.offsets == nullptr ? 1 : min(p.E, p.rows);
-  int* act_expert = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(red) + Sums<R, NT>::kBytes);
+  int* act_expert = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(red) + (split > 1 ? kWarps * kRows * kPitch * 4 : 0));
   int* act_row = act_expert + room;
   int* act_end = act_row + room;
   int* act_tile = act_end + room;
 
   // ------------------------------------------------------------ item list --
-  int routed = p.rows, active = 1;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(smem_addr(&full[i]), 1);
+      mbar_init(smem_addr(&empty[i]), kWarps);
+    }
+    abort_flag_s = 0;
+    fence_mbar_init();
+  }
+  int active = 1;
   if (p.offsets == nullptr) {
     if (threadIdx.x == 0) {
+      routed_s = p.rows;
       act_expert[0] = 0;
       act_row[0] = 0;
       act_end[0] = p.rows;
@@ -213,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) gemv_w4_kernel(cons
       act_tile[1] = (p.rows + p.tile - 1) / p.tile;
     }
   } else {
-    constexpr int kPer = kMaxExperts / kThreads;
+    constexpr int kPer = kMaxExperts / (kWarps * 32);
     int tiles[kPer], first[kPer], last[kPer], my_tiles = 0, my_act = 0, bad = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -232,10 +285,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) gemv_w4_kernel(cons
     if (__syncthreads_or(bad)) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) tiles[i] = 0;
-      my_tiles = my_act = 0;
-      routed = 0;
-    } else {
-      routed = p.offsets[p.E];
+      my_tiles = my_act = bad = 0;
+      if (threadIdx.x == 0) routed_s = 0;
+    } else if (threadIdx.x == 0) {
+      routed_s = p.offsets[p.E];
     }
     int st = my_tiles, sa = my_act;
 #pragma unroll
@@ -254,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) gemv_w4_kernel(cons
     st -= my_tiles;
     sa -= my_act;
     active = 0;
-    for (int i = 0; i < kWarps; ++i) {
+    for (int i = 0; i <= kWarps; ++i) {
       st += i < warp ? part[0][i] : 0;
       sa += i < warp ? part[1][i] : 0;
       active += part[1][i];
@@ -273,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) gemv_w4_kernel(cons
     if (threadIdx.x == kThreads - 1) act_tile[sa] = st;
   }
   __syncthreads();
-  const int ntiles = (p.N + kRows - 1) / kRows;
+  const int ntiles = (p.N + item_rows - 1) / item_rows;
   const int items = act_tile[active] * ntiles;
   const int KB = (p.K + kBlkK - 1) / kBlkK;
 
@@ -287,236 +340,235 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) gemv_w4_kernel(cons
     const int n = local / of, m = local - n * of;
     Item it;
     it.expert = act_expert[at];
-    it.n0 = n * kRows;
+    it.n0 = n * item_rows;
     it.row0 = act_row[at] + m * p.tile;
     it.count = min(p.tile, act_end[at] - it.row0);
     return it;
   };
-
-  // ------------------------------------------------------------- producer --
-  // Weights: lane -> row lane/4 + 8i, chunk lane%4.  Tokens: for at most two of
-  // them 16 lanes each, else 4 lanes each and 4 turns (and the same for tokens
-  // 8..15).  Tokens past the item's count are not copied: their columns of the
-  // MMA touch no other and are not stored.
-  const int64_t row_bytes = p.K / 2, row_step = row_bytes * 8;
-  const bool pair = p.tile <= 2;
-  const int x_tok = pair ? lane >> 4 : lane >> 2, x_chunk = pair ? lane & 15 : lane & 3;
-  const uint32_t w_dst = (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
-  const uint32_t x_dst = S::kTokenAt + x_tok * 256 + ((x_chunk ^ (4 * (x_tok & 1))) << 4);
-  const int s_per = kRows * es / 16;            // chunks of a group's scales
-  const int groups = p.K / p.G;
-  // a lane's scale chunks (at most two) and zero-point chunk within a block
-  const int64_t s_off = static_cast<int64_t>(lane / s_per) * p.N * es + (lane % s_per) * 16;
-  const int64_t s_off2 = static_cast<int64_t>((lane + 32) / s_per) * p.N * es + ((lane + 32) % s_per) * 16;
-  const int64_t z_off = static_cast<int64_t>(lane / R) * p.N + (lane % R) * 16;
-  const uint8_t *w_src = nullptr, *x_src[NT], *s_src = nullptr, *z_src = nullptr;
-  uint32_t x_size[NT];                          // 16, or 0 for a row of zeros
-  bool x_on[NT];
-  int valid16 = 0;                              // 16-row parts of the tile inside N
-  int i_item = blockIdx.x, i_kb = warp, i_at = 0;
-  uint32_t i_dst = ring;
-  auto open = [&]() {                           // the copies turn to item i_item
-    const Item in = decode(i_item, i_at);
-    valid16 = min(R, (p.N - in.n0) >> 4);
-    w_src = p.w + (static_cast<int64_t>(in.expert) * p.N + in.n0 + (lane >> 2)) * row_bytes + i_kb * (kBlkK / 2) + (lane & 3) * 16;
-    const int64_t sn = static_cast<int64_t>(in.expert) * groups * p.N + in.n0;
-    s_src = static_cast<const uint8_t*>(p.scales) + sn * es;
-    z_src = p.zeros + sn;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int m = x_tok + 8 * n;
-      x_on[n] = m < in.count;
-      x_size[n] = 0;
-      int64_t row = 0;
-      if (x_on[n]) {
-        row = in.row0 + m;
-        if (p.src != nullptr) {
-          const int from = p.src[row];
-          const bool ok = from >= 0 && from < p.rows;
-          row = ok ? from / p.topk : 0;
-          x_size[n] = ok ? 16 : 0;
-        } else {
-          x_size[n] = 16;
-        }
-      }
-      x_src[n] = static_cast<const uint8_t*>(p.x) + (row * p.ldx + i_kb * kBlkK + x_chunk * 8) * 2;
-    }
+  // x row of sorted row r, -1 where its pair is none
+  auto x_row_of = [&](int r) {
+    if (p.src == nullptr) return r;
+    const int from = p.src[r];
+    return from >= 0 && from < p.rows ? from / p.topk : -1;
   };
-  const bool busy = warp < KB;                  // has K blocks at all
-  if (busy && i_item < items) open();
-  auto issue = [&]() {
-    if (busy && i_item < items) {
-      const uint32_t s_dst = i_dst + S::scale_at(p.tile) + lane * 16, z_dst = i_dst + S::zero_at(p.tile, es) + lane * 16;
-      // a block's groups: its own 128/FL, or the one it lies in
-      const int group = FL == 128 && p.G != 128 ? i_kb / (p.G / 128) : i_kb * S::kGroups;
-      const uint8_t* sg = s_src + static_cast<int64_t>(group) * p.N * es;
-      const uint8_t* zg = z_src + static_cast<int64_t>(group) * p.N;
-      if (i_kb * kBlkK + kBlkK <= p.K && valid16 == R) {
-#pragma unroll
-        for (int i = 0; i < 2 * R; ++i) cp_async16_cg(i_dst + w_dst + i * 512, w_src + i * row_step);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (!x_on[n]) continue;
-          const uint32_t dst = i_dst + x_dst + n * (8 * 256);
-          cp_async16_cg_fill(dst, x_src[n], x_size[n]);
-          if (!pair) {
-#pragma unroll
-            for (int i = 1; i < 4; ++i) cp_async16_cg_fill(dst ^ (i << 6), x_src[n] + i * 64, x_size[n]);
-          }
+
+  int at = 0, s = 0;
+  uint32_t phase = 0;
+  if (warp == kWarps) {
+    // ----------------------------------------------------------- producer --
+    // Lane l < split brings the weights of slice l, lane 8 the scales, lane 9 the
+    // zero points, lane 16 + m the blocks of token m.  Tokens past the item's
+    // count, or without an x row, are not brought: their columns of the MMA touch
+    // no other and are not stored.
+    const uint64_t once = policy_evict_first();
+    const int groups = p.K / p.G, s_rows = split * S::kGroups;
+    int issued = 0;
+    bool gone = false;
+    for (int item = blockIdx.x; item < items && !gone; item += gridDim.x) {
+      const Item it = decode(item, at);
+      const int x_row = lane >= 16 && lane - 16 < it.count ? x_row_of(it.row0 + lane - 16) : -1;
+      const int x_rows = __popc(__ballot_sync(0xffffffffu, x_row >= 0));
+      const uint8_t* x = static_cast<const uint8_t*>(p.x) + (x_row < 0 ? 0 : x_row) * p.ldx * 2;
+      for (int kb = 0; kb < KB; kb += split) {
+        const bool ok = wait_bounded(smem_addr(&empty[s]), phase ^ 1u, abort_flag, p.status, kStW4, p.timeout_ns);
+        if (!__all_sync(0xffffffffu, ok)) {
+          gone = true;
+          break;
         }
-        if (lane < S::kGroups * s_per) cp_async16_cg(s_dst, sg + s_off);
-        if (S::kGroups * R * 4 > 32 && lane + 32 < S::kGroups * s_per) cp_async16_cg(s_dst + 512, sg + s_off2);
-        if (ZP && lane < S::kGroups * R) cp_async16_cg(z_dst, zg + z_off);
-      } else {
-        const int left = p.K - i_kb * kBlkK;    // k of this block inside K
-#pragma unroll
-        for (int i = 0; i < 2 * R; ++i) {
-          const bool ok = (i >> 1) < valid16 && (lane & 3) * 32 < left;
-          cp_async16_cg_fill(i_dst + w_dst + i * 512, ok ? w_src + i * row_step : p.w, ok ? 16u : 0u);
+        const uint32_t bar = smem_addr(&full[s]), dst = ring + s * stage_bytes;
+        const int blocks = min(split, KB - kb);
+        const uint32_t x_bytes = min(split * kBlkK, p.K - kb * kBlkK) * 2;
+        if (lane == 0)
+          mbar_arrive_expect_tx(bar, blocks * item_rows * 64 + boxes * s_rows * box_rows * (es + (ZP ? 1 : 0)) + x_rows * x_bytes);
+        __syncwarp();
+        const int group = it.expert * groups + (FL == 128 ? kb * kBlkK / p.G : kb * S::kGroups);
+        if (lane < blocks) {
+          for (int b = 0; b < boxes; ++b)
+            tma_load_2d(dst + lane * item_rows * 64 + b * box_rows * 64, &w_map, bar, (kb + lane) * (kBlkK / 2),
+                        it.expert * p.N + it.n0 + b * box_rows, once);
+        } else if (lane == 8) {
+          for (int b = 0; b < boxes; ++b)
+            tma_load_2d(dst + scale_at + b * scale_box, &s_map, bar, it.n0 + b * box_rows, group, once);
+        } else if (ZP && lane == 9) {
+          for (int b = 0; b < boxes; ++b)
+            tma_load_2d(dst + zero_at + b * zero_box, &z_map, bar, it.n0 + b * box_rows, group, once);
+        } else if (x_row >= 0) {
+          bulk_load_1d(dst + S::kWeightBytes + (lane - 16) * x_pitch, x + static_cast<int64_t>(kb) * (kBlkK * 2), x_bytes, bar);
         }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (!x_on[n]) continue;
-          const uint32_t dst = i_dst + x_dst + n * (8 * 256);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (pair && i) break;
-            const bool ok = x_chunk * 8 + i * 32 < left;
-            cp_async16_cg_fill(dst ^ (i << 6), ok ? x_src[n] + i * 64 : p.x, ok ? x_size[n] : 0u);
-          }
+        __syncwarp();
+        ++issued;
+        if (++s == p.stages) {
+          s = 0;
+          phase ^= 1u;
         }
-        for (int i = lane; i < S::kGroups * s_per; i += 32) {
-          const int gi = i / s_per, c = i - gi * s_per;
-          const bool ok = group + gi < groups && (c * (16 / es)) >> 4 < valid16;
-          cp_async16_cg_fill(s_dst + (i - lane) * 16, ok ? sg + static_cast<int64_t>(gi) * p.N * es + c * 16 : p.scales,
-                             ok ? 16u : 0u);
-        }
-        if (ZP && lane < S::kGroups * R) {
-          const bool ok = group + lane / R < groups && lane % R < valid16;
-          cp_async16_cg_fill(z_dst, ok ? zg + z_off : p.zeros, ok ? 16u : 0u);
-        }
-      }
-      i_dst = i_dst + stage_bytes == ring + STAGES * stage_bytes ? ring : i_dst + stage_bytes;
-      i_kb += kWarps;
-      w_src += kWarps * (kBlkK / 2);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) x_src[n] += kWarps * kBlkK * 2;
-      if (i_kb >= KB) {
-        i_kb = warp;
-        i_item += gridDim.x;
-        if (i_item < items) open();
       }
     }
-    cp_async_commit();                          // one group a step, empty past the end, so the counts hold
-  };
+    if (gone && lane == 0) {
+      // no copy may land after the CTA exits: wait (bounded, fresh deadline) for the last stages issued
+      volatile int no_abort = 0;
+      for (int i = issued > p.stages ? issued - p.stages : 0; i < issued; ++i)
+        wait_bounded(smem_addr(&full[i % p.stages]), (i / p.stages) & 1u, &no_abort, p.status, kStW4, p.timeout_ns);
+    }
+    __syncwarp();
+  } else {
+    // ----------------------------------------------------------- consumer --
+    // A wait that gave up leaves the control flow as it is (the barriers below
+    // count on every warp) and the status word says that the result is none.
+    const int slice = warp % split, part_no = warp / split;
+    const int box = part_no * kRows / box_rows, box_row = part_no * kRows - box * box_rows;
+    const uint32_t w_at = slice * item_rows * 64 + (part_no * kRows + g) * 64 +
+                          (((S::kWords == 1 ? 0 : S::kWords == 2 ? q >> 1 : q) ^ ((g >> 1) & 3)) << 4) +
+                          (S::kWords == 1 ? q * 4 : S::kWords == 2 ? (q & 1) * 8 : 0);
+    // lanes whose token the tile does not have read another's: their columns are not stored
+    uint32_t x_at[NT];
 #pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) issue();
-
-  // ------------------------------------------------------------- consumer --
-  const uint32_t w_at = g * 64 + (((g >> 1) & 3) << 4) + q * 4;         // ^ 16j
-  const uint32_t x_at = S::kTokenAt + g * 256 + ((g & 1) << 6) + q * 16;  // ^ 64j
-  int c_at = 0;
-  uint32_t st = ring;
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    const Item it = decode(item, c_at);
-    float acc[R][NT][4];
+    for (int n = 0; n < NT; ++n)
+      x_at[n] = S::kWeightBytes + min(8 * n + g, p.tile - 1) * x_pitch + slice * 256 + S::kWords * q * 16;
+    const uint32_t s_at = scale_at + box * scale_box + (box_row + g) * es, z_at = zero_at + box * zero_box + box_row + g;
+    bool alive = true;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+      const Item it = decode(item, at);
+      float acc[R][NT][4];
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+      for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.0f;
-    for (int kb = warp; kb < KB; kb += kWarps) {
-      __syncwarp();                             // every lane has read the stage that is refilled next
-      issue();
-      cp_async_wait<STAGES - 1>();              // this lane's copies of the block have landed ...
-      __syncwarp();                             // ... and every other lane's
-      float d[R][NT][4];
-      uint32_t mz[R][2];                        // minus the zero points of rows g, g + 8
+          for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.0f;
+      for (int kb0 = 0; kb0 < KB; kb0 += split) {
+        if (alive) alive = wait_bounded(smem_addr(&full[s]), phase, abort_flag, p.status, kStW4, p.timeout_ns);
+        __syncwarp();
+        const int kb = kb0 + slice;
+        if (kb < KB) {
+          const uint32_t st = ring + s * stage_bytes;
+          const int left = p.K - kb * kBlkK;    // k of this block inside K
+          // the block's first row of scales: its own, or that of the group it lies in
+          int srow = slice * S::kGroups;
+          if (FL == 128 && p.G != 128)
+            srow = kb * kBlkK / p.G - kb0 * kBlkK / p.G;
+          float d[R][NT][4];
+          uint32_t mz[R][2];                    // minus the zero points of rows g, g + 8
+          uint32_t wl[R][S::kWords], wh[R][S::kWords];   // their words
+#pragma unroll (FL < 128 && R == 4 && NT == 1 && ZP ? FL / 32 : 4)
+          for (int j = 0; j < 4; ++j) {         // 32 k each
+            const bool first = j * 32 % FL == 0;
+            if (first) {
+              const uint32_t zp = st + z_at + (srow + j * 32 / FL) * box_rows;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {             // 32 k each
-        const bool first = j * 32 % FL == 0;
-        if (first) {
-          const uint32_t zp = st + S::zero_at(p.tile, es) + (j * 32 / FL) * kRows + g;
+              for (int r = 0; r < R; ++r) {
+                mz[r][0] = mz[r][1] = C::kMinusEight;
+                if (ZP) {
+                  mz[r][0] = mul2<T>((lds8(zp + r * 16) & 15u) * 0x00010001u, C::kNegate);
+                  mz[r][1] = mul2<T>((lds8(zp + r * 16 + 8) & 15u) * 0x00010001u, C::kNegate);
+                }
+              }
+            }
+            const int chunk = 4 * S::kWords * (j / S::kWords) + j % S::kWords;   // + WV q: the lane's 8 k
+            uint32_t b[NT][4];
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            mz[r][0] = mz[r][1] = C::kMinusEight;
-            if (ZP) {
-              mz[r][0] = mul2<T>((lds8(zp + r * 16) & 15u) * 0x00010001u, C::kNegate);
-              mz[r][1] = mul2<T>((lds8(zp + r * 16 + 8) & 15u) * 0x00010001u, C::kNegate);
+            for (int n = 0; n < NT; ++n) {
+              uint4 v = lds128(st + x_at[n] + chunk * 16);
+              if (FL < 128 && (chunk + S::kWords * q) * 8 >= left) v = make_uint4(0, 0, 0, 0);   // past K: not brought
+              b[n][0] = __byte_perm(v.x, v.z, 0x5410);      // x0, x4
+              b[n][1] = __byte_perm(v.x, v.z, 0x7632);      // x1, x5
+              b[n][2] = __byte_perm(v.y, v.w, 0x5410);      // x2, x6
+              b[n][3] = __byte_perm(v.y, v.w, 0x7632);      // x3, x7
+            }
+            if (j % S::kWords == 0) {
+              // part j / WV: 16 bytes on (WV = 1), 32 bytes on (WV = 2)
+              const uint32_t wj = (st + w_at) ^ (S::kWords == 1 ? j << 4 : S::kWords == 2 ? (j >> 1) << 5 : 0);
+#pragma unroll
+              for (int r = 0; r < R; ++r) {
+                lds_words(wj + r * 1024, wl[r]);
+                lds_words(wj + r * 1024 + 512, wh[r]);
+              }
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+              uint32_t l[4], h[4];
+              unpack_codes<T>(wl[r][j % S::kWords], mz[r][0], l);
+              unpack_codes<T>(wh[r][j % S::kWords], mz[r][1], h);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                mma_step<T>(d[r][n], first, l[0], h[0], l[1], h[1], b[n][0], b[n][1]);
+                mma_step<T>(d[r][n], false, l[2], h[2], l[3], h[3], b[n][2], b[n][3]);
+              }
+            }
+            if ((j + 1) * 32 % FL == 0) {
+              const uint32_t sp = st + s_at + (srow + j * 32 / FL) * box_rows * es;
+              float scale[R][2];
+              if (p.scale_f32) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                  scale[r][0] = __uint_as_float(lds32(sp + r * 64));
+                  scale[r][1] = __uint_as_float(lds32(sp + r * 64 + 32));
+                }
+              } else {
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                  scale[r][0] = scale_of(lds16(sp + r * 32), static_cast<T*>(nullptr));
+                  scale[r][1] = scale_of(lds16(sp + r * 32 + 16), static_cast<T*>(nullptr));
+                }
+              }
+#pragma unroll
+              for (int r = 0; r < R; ++r) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) acc[r][n][i] = fmaf(scale[r][i / 2], d[r][n][i], acc[r][n][i]);
+              }
             }
           }
         }
-        uint32_t b[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (8 * n + g < p.tile) v = lds128((st + x_at + n * (8 * 256)) ^ (j << 6));
-          b[n][0] = __byte_perm(v.x, v.z, 0x5410);          // x0, x4
-          b[n][1] = __byte_perm(v.x, v.z, 0x7632);          // x1, x5
-          b[n][2] = __byte_perm(v.y, v.w, 0x5410);          // x2, x6
-          b[n][3] = __byte_perm(v.y, v.w, 0x7632);          // x3, x7
+        __syncwarp();                           // every lane has read the stage
+        if (lane == 0) mbar_arrive(smem_addr(&empty[s]));
+        if (++s == p.stages) {
+          s = 0;
+          phase ^= 1u;
         }
-        const uint32_t wj = (st + w_at) ^ (j << 4);
+      }
+      const unsigned rows_with_x = __ballot_sync(0xffffffffu, lane < it.count && x_row_of(it.row0 + lane) >= 0);
+      T* y = static_cast<T*>(p.y) + static_cast<int64_t>(it.row0) * p.ldy;
+      if (split == 1) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          uint32_t l[4], h[4];
-          unpack_codes<T>(lds32(wj + r * 1024), mz[r][0], l);
-          unpack_codes<T>(lds32(wj + r * 1024 + 512), mz[r][1], h);
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int m = 8 * n + 2 * q + (i & 1), row = it.n0 + part_no * kRows + 16 * r + g + (i < 2 ? 0 : 8);
+              if (m < it.count && row < p.N)
+                y[static_cast<int64_t>(m) * p.ldy + row] = C::from(rows_with_x >> m & 1u ? acc[r][n][i] * C::kScale : 0.0f);
+            }
+      } else {
+        // the slices' partial sums, added in slice order
+        float* mine = red + warp * (kRows * kPitch);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            mma_step<T>(d[r][n], first, l[0], h[0], l[1], h[1], b[n][0], b[n][1]);
-            mma_step<T>(d[r][n], false, l[2], h[2], l[3], h[3], b[n][2], b[n][3]);
+            float* lo = mine + (16 * r + g) * kPitch + 8 * n + 2 * q;
+            float* hi = lo + 8 * kPitch;
+            lo[0] = acc[r][n][0];
+            lo[1] = acc[r][n][1];
+            hi[0] = acc[r][n][2];
+            hi[1] = acc[r][n][3];
           }
+        bar_sync(1, kWarps * 32);
+        for (int o = threadIdx.x; o < item_rows * it.count; o += kWarps * 32) {
+          const int m = o / item_rows, row = o - m * item_rows;
+          const float* f = red + ((row / kRows) * split * kRows + row % kRows) * kPitch + m;
+          float v = 0.0f;
+          for (int w = 0; w < split; ++w) v += f[w * (kRows * kPitch)];
+          if (it.n0 + row < p.N)
+            y[static_cast<int64_t>(m) * p.ldy + it.n0 + row] = C::from(rows_with_x >> m & 1u ? v * C::kScale : 0.0f);
         }
-        if ((j + 1) * 32 % FL == 0) {
-          const uint32_t sp = st + S::scale_at(p.tile) + ((j * 32 / FL) * kRows + g) * es;
-#pragma unroll
-          for (int r = 0; r < R; ++r) {
-            float sl, sh;
-            if (p.scale_f32) {
-              sl = __uint_as_float(lds32(sp + r * 64));
-              sh = __uint_as_float(lds32(sp + r * 64 + 32));
-            } else {
-              sl = scale_of(lds16(sp + r * 32), static_cast<T*>(nullptr));
-              sh = scale_of(lds16(sp + r * 32 + 16), static_cast<T*>(nullptr));
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) acc[r][n][i] = fmaf(i < 2 ? sl : sh, d[r][n][i], acc[r][n][i]);
-          }
-        }
+        bar_sync(1, kWarps * 32);               // the partial sums may be overwritten
       }
-      st = st + stage_bytes == ring + STAGES * stage_bytes ? ring : st + stage_bytes;
     }
-    // the warps' partial sums, added in warp order
-    float* mine = red + warp * (kRows * kPitch);
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float* lo = mine + (16 * r + g) * kPitch + 8 * n + 2 * q;
-        float* hi = lo + 8 * kPitch;
-        lo[0] = acc[r][n][0];
-        lo[1] = acc[r][n][1];
-        hi[0] = acc[r][n][2];
-        hi[1] = acc[r][n][3];
-      }
-    __syncthreads();
-    for (int o = threadIdx.x; o < kRows * it.count; o += kThreads) {
-      const int m = o / kRows, row = o - m * kRows;
-      float s = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) s += red[(w * kRows + row) * kPitch + m];
-      if (it.n0 + row < p.N)
-        static_cast<T*>(p.y)[static_cast<int64_t>(it.row0 + m) * p.ldy + it.n0 + row] = C::from(s * C::kScale);
-    }
-    __syncthreads();                            // the partial sums may be overwritten
   }
-  cp_async_wait<0>();
   // rows of no expert
-  for (int64_t r = routed + static_cast<int64_t>(blockIdx.x); r < p.rows; r += gridDim.x)
+  for (int64_t r = routed_s + static_cast<int64_t>(blockIdx.x); r < p.rows; r += gridDim.x)
     for (int n = threadIdx.x; n < p.N; n += kThreads) static_cast<T*>(p.y)[r * p.ldy + n] = C::from(0.0f);
 }
 
@@ -525,15 +577,55 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) gemv_w4_kernel(cons
 static bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 constexpr int kMaxDevices = 64;
-constexpr int kSmemMost = 226 * 1024;
+constexpr int kSmemMost = 226 * 1024, kSmemPair = 112 * 1024;   // a CTA alone on its SM, or one of two
 static std::mutex g_mu;
 
-template <typename T, int R, int NT, int FL, bool ZP, int STAGES>
-static int launch(const Args& a, int sms, cudaStream_t s) {
-  const auto kernel = gemv_w4_kernel<T, R, NT, FL, ZP, STAGES>;
+// A plan: rows of a warp (16R), slices of K, and what it is thought to take.
+struct Plan {
+  int R, split;
+  double us;
+};
+
+// The cheapest R and split for `tiles` token tiles of up to 8 NT tokens.  Measured
+// on B200, microseconds: a step of an item (one K block a warp) costs an SM 0.56
+// (R = 2) or 0.95 (R = 4) with 8 tokens and two CTAs on it, 0.93 or 1.65 with 16 and one
+// CTA; one CTA of two alone takes 1.6 times as long for its own;
+// joining the slices of an item costs 1.0 (R = 2) or 1.7 (R = 4) with eight, 0.8
+// with two or four, 0.3 with one.  (65536 x 7168, one token: R = 4 with two slices
+// 58 us, R = 2 with one 63; 7168 x 2048: R = 2 with eight slices 11.2, R = 4 12.3;
+// 8192 x 7168, 16 tokens: R = 4 22, R = 2 29.)
+static Plan plan(int NT, double tiles, int N, int K, int sms) {
+  Plan best = {2, kWarps, 1e30};
+  const int KB = (K + kBlkK - 1) / kBlkK;
+  for (int R = 2; R <= 4; R += 2) {
+    const double step = NT == 1 ? (R == 2 ? 0.56 : 0.95) : (R == 2 ? 0.93 : 1.65);
+    const int ctas = NT == 1 ? 2 : 1;
+    for (int split = kWarps; split >= 1; split /= 2) {
+      const int rows = 16 * R * (kWarps / split), steps = (KB + split - 1) / split;
+      const double items = tiles * ((N + rows - 1) / rows);
+      const double join = split == kWarps ? (R == 2 ? 1.0 : 1.7) : split > 1 ? 0.8 : 0.3;
+      const double busy = ceil(items / sms) * (steps * step + join);
+      const double alone = ceil(items / (sms * ctas)) * (0.8 * ctas * steps * step + join);
+      const double us = busy > alone ? busy : alone;
+      if (us < best.us) best = {R, split, us};
+    }
+  }
+  return best;
+}
+
+template <typename T, int R, int NT, int FL, bool ZP>
+static int launch(Args& a, int sms, cudaStream_t s) {
+  using S = Stage<R, FL>;
+  const auto kernel = gemv_w4_kernel<T, R, NT, FL, ZP>;
+  const int es = a.scale_f32 ? 4 : 2;
   const int room = a.offsets ? (a.E < a.rows ? a.E : a.rows) : 1;
-  const int smem = kWarps * STAGES * Stage<R, FL>::bytes(a.tile, a.scale_f32 ? 4 : 2, ZP) + Sums<R, NT>::kBytes +
-                   (4 * room + 1) * static_cast<int>(sizeof(int));
+  const int stage = S::bytes(a.tile, a.split, es, ZP);
+  const int rest = Sums<R, NT>::bytes(a.split) + (4 * room + 1) * static_cast<int>(sizeof(int));
+  const bool pair = NT == 1 && rest + 2 * stage <= kSmemPair;
+  a.stages = ((pair ? kSmemPair : kSmemMost) - rest) / stage;
+  if (a.stages > kMaxStages) a.stages = kMaxStages;
+  if (a.stages < 1) return record_error(FACK_ERR_LAUNCH, "the 4-bit kernel's stage does not fit an SM");
+  const int smem = a.stages * stage + rest;
   int dev = 0, per_sm = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return FACK_ERR_CUDA;
   {
@@ -550,33 +642,78 @@ static int launch(const Args& a, int sms, cudaStream_t s) {
     }
     per_sm = last[dev][1];
   }
+  const int64_t rows = S::kRows * (kWarps / a.split), ntiles = (a.N + rows - 1) / rows, slots = static_cast<int64_t>(sms) * per_sm;
   // at most this many items: every expert with rows starts one token tile, every a.tile rows fill one
-  const int64_t ntiles = (a.N + 16 * R - 1) / (16 * R);
   const int64_t most = (a.rows / a.tile + static_cast<int64_t>(room) + 1) * ntiles;
-  if (most > INT32_MAX) return FACK_ERR_BAD_SHAPE;
-  const int64_t grid = most < static_cast<int64_t>(sms) * per_sm ? most : static_cast<int64_t>(sms) * per_sm;
-  kernel<<<static_cast<unsigned>(grid), kThreads, smem, s>>>(a);
+  if (most > INT32_MAX - slots) return FACK_ERR_BAD_SHAPE;
+  CUtensorMap wm, sm, zm;
+  const uint64_t E = a.E, N = a.N, K = a.K, groups = a.K / a.G;
+  int st = encode_elems_2d(&wm, a.w, 1, K / 2, E * N, K / 2, kBlkK / 2, S::box_rows(a.split), true);
+  if (st == FACK_OK)
+    st = encode_elems_2d(&sm, a.scales, es, N, E * groups, N * es, S::box_rows(a.split), a.split * S::kGroups, false);
+  if (st == FACK_OK) {
+    if (ZP)
+      st = encode_elems_2d(&zm, a.zeros, 1, N, E * groups, N, S::box_rows(a.split), a.split * S::kGroups, false);
+    else
+      zm = sm;                                  // not used
+  }
+  if (st != FACK_OK) return record_error(st, "the tensor map of the 4-bit weight was refused");
+  kernel<<<static_cast<unsigned>(most < slots ? most : slots), kThreads, smem, s>>>(wm, sm, zm, a);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? FACK_OK : record_error(FACK_ERR_LAUNCH, cudaGetErrorString(e));
 }
 
 template <typename T, int FL, bool ZP>
-static int by_tokens(Args& a, int per_expert, int tokens, int sms, cudaStream_t s) {
-  if (per_expert <= 8) {
-    a.tile = tokens < 8 ? tokens : 8;
-    return a.tile <= 2 ? launch<T, 2, 1, FL, ZP, 4>(a, sms, s) : launch<T, 2, 1, FL, ZP, 3>(a, sms, s);
-  }
-  a.tile = tokens < 16 ? tokens : 16;
-  return launch<T, 4, 2, FL, ZP, 2>(a, sms, s);
+static int by_plan(Args& a, int NT, int R, int sms, cudaStream_t s) {
+  if (NT == 1) return R == 2 ? launch<T, 2, 1, FL, ZP>(a, sms, s) : launch<T, 4, 1, FL, ZP>(a, sms, s);
+  return R == 2 ? launch<T, 2, 2, FL, ZP>(a, sms, s) : launch<T, 4, 2, FL, ZP>(a, sms, s);
 }
 
 template <typename T, bool ZP>
-static int by_group(Args& a, int per_expert, int tokens, int sms, cudaStream_t s) {
-  if (a.G % 128 == 0) return by_tokens<T, 128, ZP>(a, per_expert, tokens, sms, s);
-  return a.G == 64 ? by_tokens<T, 64, ZP>(a, per_expert, tokens, sms, s) : by_tokens<T, 32, ZP>(a, per_expert, tokens, sms, s);
+static int by_group(Args& a, int NT, int R, int sms, cudaStream_t s) {
+  if (a.G % 128 == 0) return by_plan<T, 128, ZP>(a, NT, R, sms, s);
+  return a.G == 64 ? by_plan<T, 64, ZP>(a, NT, R, sms, s) : by_plan<T, 32, ZP>(a, NT, R, sms, s);
 }
 
-static int run(Args& a, int dtype, int scale_dtype, int per_expert, int tokens, void* stream) {
+// Token tiles that `rows` rows, sent to E experts at random, are expected to take:
+// E times the mean of ceil(x / tile) over a Poisson x.
+static double expected_tiles(int64_t rows, int E, int tile) {
+  const double mean = static_cast<double>(rows) / E;
+  if (mean > 200.0) return E * (mean / tile + 0.5);
+  double sum = 0.0, p = exp(-mean);
+  for (int x = 1; x < 600; ++x) {
+    p *= mean / x;
+    sum += p * ((x + tile - 1) / tile);
+  }
+  return E * sum;
+}
+
+// Tokens per tile (8 NT at most) and the plan.  An expert's rows are known on the
+// device alone; it is not likely to have more than there are tokens.
+static void choose(Args& a, int tokens, int sms, int* NT, int* R) {
+  Plan p[2];
+  int tile[2];
+  for (int i = 0; i < 2; ++i) {
+    const int most = 8 * (i + 1);
+    double tiles;
+    if (a.offsets) {
+      tile[i] = tokens < most ? tokens : most;
+      tiles = expected_tiles(a.rows, a.E, tile[i]);
+    } else {
+      const int64_t n = (static_cast<int64_t>(a.rows) + most - 1) / most;
+      tile[i] = static_cast<int>((a.rows + n - 1) / n);      // evenly filled
+      tiles = static_cast<double>(n);
+    }
+    p[i] = plan(i + 1, tiles, a.N, a.K, sms);
+  }
+  const int i = tile[1] > 8 && p[1].us < p[0].us;
+  *NT = i + 1;
+  *R = p[i].R;
+  a.tile = tile[i];
+  a.split = p[i].split;
+}
+
+static int run(Args& a, int dtype, int scale_dtype, int tokens, void* stream) {
   if (a.rows < 1 || a.N < 16 || a.N % 16 || a.N > (1 << 24) || a.K < 32 || a.K > (1 << 20)) return FACK_ERR_BAD_SHAPE;
   if ((a.G != 32 && a.G != 64 && (a.G < 128 || a.G % 128)) || a.K % a.G) return FACK_ERR_BAD_ARG;
   if (dtype != FACK_DTYPE_BF16 && dtype != FACK_DTYPE_F16) return FACK_ERR_BAD_ARG;
@@ -589,11 +726,18 @@ static int run(Args& a, int dtype, int scale_dtype, int per_expert, int tokens, 
   const int st = sm100_device(&sms);
   if (st != FACK_OK) return st;
   a.scale_f32 = scale_dtype == FACK_DTYPE_F32;
+  a.status = device_status_word();
+  a.timeout_ns = 2000000000ull;                // 2 s
+  if (!a.status) return FACK_ERR_CUDA;
+  // the copies count rows in 32 bits
+  if (static_cast<int64_t>(a.E) * a.N > INT32_MAX - 1024 || static_cast<int64_t>(a.E) * (a.K / a.G) > INT32_MAX - 1024)
+    return FACK_ERR_BAD_SHAPE;
+  int NT, R;
+  choose(a, tokens, sms, &NT, &R);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == FACK_DTYPE_BF16)
-    return a.zeros ? by_group<__nv_bfloat16, true>(a, per_expert, tokens, sms, s)
-                   : by_group<__nv_bfloat16, false>(a, per_expert, tokens, sms, s);
-  return a.zeros ? by_group<__half, true>(a, per_expert, tokens, sms, s) : by_group<__half, false>(a, per_expert, tokens, sms, s);
+    return a.zeros ? by_group<__nv_bfloat16, true>(a, NT, R, sms, s) : by_group<__nv_bfloat16, false>(a, NT, R, sms, s);
+  return a.zeros ? by_group<__half, true>(a, NT, R, sms, s) : by_group<__half, false>(a, NT, R, sms, s);
 }
 
 }  // namespace fack_w4
@@ -617,7 +761,7 @@ int fack_gemv_w4(const void* x, int dtype, int64_t ldx, const void* w, const voi
   a.K = K;
   a.G = group;
   a.E = 1;
-  return run(a, dtype, scale_dtype, M, M, stream);
+  return run(a, dtype, scale_dtype, M, stream);
 }
 
 int fack_gemv_w4_experts(const void* x, int dtype, int64_t ldx, const void* w, const void* scales, int scale_dtype,
@@ -644,7 +788,7 @@ int fack_gemv_w4_experts(const void* x, int dtype, int64_t ldx, const void* w, c
   a.K = K;
   a.G = group;
   a.E = num_experts;
-  return run(a, dtype, scale_dtype, (a.rows + num_experts - 1) / num_experts, T, stream);
+  return run(a, dtype, scale_dtype, T, stream);
 }
 
 }  // extern "C"
