@@ -23,10 +23,11 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .ops import BLOCK, FP8, _stream_handle
+from .ops import BLOCK, FP8
 
 MAX_EXPERTS = 1024
 MAX_TOPK = 64
+SORT_ONE_BLOCK = 512     # pairs that one block always sorts, without a workspace
 
 DTYPES = {torch.float32: _lib.FACK_DTYPE_F32, torch.bfloat16: _lib.FACK_DTYPE_BF16,
           torch.float16: _lib.FACK_DTYPE_F16}
@@ -45,22 +46,20 @@ class MoePlan(NamedTuple):
     offsets: torch.Tensor
 
 
-class _on:
-    """The device made current for a call, unless it is already."""
-    __slots__ = ("index", "guard")
+def _call(name: str, dev: torch.device, *args) -> None:
+    """One C entry on ``dev``'s current stream, with ``dev`` current meanwhile.
 
-    def __init__(self, dev):
-        self.index = dev.index
-        self.guard = None
-
-    def __enter__(self):
-        if torch.cuda.current_device() != self.index:
-            self.guard = torch.cuda.device(self.index)
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+    A decode step makes these calls for microseconds of GPU work each, so the
+    host's share is kept small: the stream's handle is read without making a
+    stream object, and the device is switched only when it has to be."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == dev.index:
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if st:
+        _lib.check(st, name)
 
 
 def _check_plan(plan, dev: torch.device):
@@ -114,63 +113,80 @@ def moe_sort(topk_ids: torch.Tensor, num_experts: int) -> MoePlan:
         raise ValueError(f"moe_sort takes 1 to {MAX_TOPK} slots, 1 to {MAX_EXPERTS} experts and fewer than 2^31 pairs")
     dev = topk_ids.device
     ids = topk_ids.contiguous()
-    row_of = torch.empty((T, topk), dtype=torch.int32, device=dev)
-    src = torch.empty((T * topk,), dtype=torch.int32, device=dev)
+    row_of = ids.new_empty((T, topk), dtype=torch.int32)
+    src = ids.new_empty((T * topk,), dtype=torch.int32)
     if T == 0:
-        return MoePlan(row_of, src, torch.zeros((E + 1,), dtype=torch.int32, device=dev))
-    offsets = torch.empty((E + 1,), dtype=torch.int32, device=dev)
-    lib = _lib.load()
-    nb = ctypes.c_size_t()
-    _lib.check(lib.fack_moe_sort_workspace_size(T, topk, E, ctypes.byref(nb)), "fack_moe_sort_workspace_size")
-    # of this call alone: two captured sorts, or two streams, never share one
-    ws = torch.empty((nb.value,), dtype=torch.uint8, device=dev) if nb.value else None
-    with _on(dev):
-        st = lib.fack_moe_sort(ids.data_ptr(), ids.element_size(), T, topk, E, row_of.data_ptr(), src.data_ptr(),
-                               offsets.data_ptr(), None if ws is None else ws.data_ptr(), nb.value,
-                               _stream_handle(dev))
-    _lib.check(st, "fack_moe_sort")
+        return MoePlan(row_of, src, ids.new_zeros((E + 1,), dtype=torch.int32))
+    offsets = ids.new_empty((E + 1,), dtype=torch.int32)
+    ws, nb = None, 0
+    if T * topk > SORT_ONE_BLOCK:
+        size = ctypes.c_size_t()
+        _lib.check(_lib.load().fack_moe_sort_workspace_size(T, topk, E, ctypes.byref(size)),
+                   "fack_moe_sort_workspace_size")
+        nb = size.value
+        # of this call alone: two captured sorts, or two streams, never share one
+        ws = ids.new_empty((nb,), dtype=torch.uint8) if nb else None
+    _call("fack_moe_sort", dev, ids.data_ptr(), ids.element_size(), T, topk, E, row_of.data_ptr(), src.data_ptr(),
+          offsets.data_ptr(), None if ws is None else ws.data_ptr(), nb)
     return MoePlan(row_of, src, offsets)
 
 
 def _gather(x, plan):
     _check_rows(x, "x")
-    dev = x.device
-    T, topk, E = _check_plan(plan, dev)
-    D = x.shape[1]
+    T, topk, E = _check_plan(plan, x.device)
     if x.shape[0] != T:
         raise ValueError(f"x has {x.shape[0]} rows, the plan {T} tokens")
-    y = torch.empty((T * topk, D), dtype=x.dtype, device=dev)
+    D = x.shape[1]
+    y = x.new_empty((T * topk, D))
     if T:
-        with _on(dev):
-            st = _lib.load().fack_moe_gather(x.data_ptr(), DTYPES[x.dtype], _ld(x), T, topk, D,
-                                             plan.row_of.data_ptr(), plan.offsets.data_ptr(), E, y.data_ptr(), D,
-                                             _stream_handle(dev))
-        _lib.check(st, "fack_moe_gather")
+        _call("fack_moe_gather", x.device, x.data_ptr(), DTYPES[x.dtype], _ld(x), T, topk, D, plan.row_of.data_ptr(),
+              plan.offsets.data_ptr(), E, y.data_ptr(), D)
     return y
 
 
-def _combine(y, weights, plan):
-    _check_rows(y, "y")
-    dev = y.device
-    T, topk, _ = _check_plan(plan, dev)
+def _sum_rows(y, w, row_of):
+    """The combine kernel on checked operands (w None: ones)."""
+    T, topk = row_of.shape
     D = y.shape[1]
+    out = y.new_empty((T, D))
+    if T:
+        _call("fack_moe_combine", y.device, y.data_ptr(), DTYPES[y.dtype], _ld(y), None if w is None else w.data_ptr(),
+              T, topk, D, row_of.data_ptr(), out.data_ptr(), D)
+    return out
+
+
+def _check_sorted(y, plan):
+    _check_rows(y, "y")
+    T, topk, _ = _check_plan(plan, y.device)
     if y.shape[0] != T * topk:
         raise ValueError(f"y has {y.shape[0]} rows, the plan {T * topk}")
-    w = None if weights is None else _check_weights(weights, T, topk, dev)
-    out = torch.empty((T, D), dtype=y.dtype, device=dev)
-    if T:
-        with _on(dev):
-            st = _lib.load().fack_moe_combine(y.data_ptr(), DTYPES[y.dtype], _ld(y), None if w is None else w.data_ptr(),
-                                              T, topk, D, plan.row_of.data_ptr(), out.data_ptr(), D,
-                                              _stream_handle(dev))
-        _lib.check(st, "fack_moe_combine")
-    return out
+    return T, topk
+
+
+def _combine(y, weights, plan):
+    T, topk = _check_sorted(y, plan)
+    return _sum_rows(y, _check_weights(weights, T, topk, y.device), plan.row_of)
 
 
 def moe_gather_backward(dy: torch.Tensor, plan: MoePlan) -> torch.Tensor:
     """dx [T, D] of :func:`moe_gather` from dy [T*k, D]: each token's rows
     summed in fp32, slots in order, rounded once."""
-    return _combine(dy, None, plan)
+    _check_sorted(dy, plan)
+    return _sum_rows(dy, None, plan.row_of)
+
+
+def _combine_grads(dout, y, w, row_of, offsets, need_dy, need_dw):
+    """The gradient kernel on checked operands (y is read for dw alone)."""
+    T, topk = row_of.shape
+    D = dout.shape[1]
+    dy = dout.new_empty((T * topk, D)) if need_dy else None
+    dw = dout.new_empty((T, topk), dtype=torch.float32) if need_dw else None
+    if T and (need_dy or need_dw):
+        _call("fack_moe_combine_bwd", dout.device, dout.data_ptr(), DTYPES[dout.dtype], _ld(dout),
+              y.data_ptr() if need_dw else None, _ld(y) if need_dw else 0, w.data_ptr(), T, topk, D,
+              row_of.data_ptr(), offsets.data_ptr(), offsets.shape[0] - 1, dy.data_ptr() if need_dy else None, D,
+              dw.data_ptr() if need_dw else None)
+    return dy, dw
 
 
 def moe_combine_backward(dout: torch.Tensor, y: Optional[torch.Tensor], weights: torch.Tensor, plan: MoePlan,
@@ -180,26 +196,15 @@ def moe_combine_backward(dout: torch.Tensor, y: Optional[torch.Tensor], weights:
     without ``need_dweights``).  Rows of dy without a pair are zero."""
     _check_rows(dout, "dout")
     dev = dout.device
-    T, topk, E = _check_plan(plan, dev)
-    D = dout.shape[1]
+    T, topk, _ = _check_plan(plan, dev)
     if dout.shape[0] != T:
         raise ValueError(f"dout has {dout.shape[0]} rows, the plan {T} tokens")
     w = _check_weights(weights, T, topk, dev)
     if need_dweights:
-        _check_rows(y, "y", T * topk, D)
+        _check_rows(y, "y", T * topk, dout.shape[1])
         if y.dtype != dout.dtype or y.device != dev:
             raise ValueError("y and dout must have one type and device")
-    dy = torch.empty((T * topk, D), dtype=dout.dtype, device=dev) if need_dy else None
-    dw = torch.empty((T, topk), dtype=torch.float32, device=dev) if need_dweights else None
-    if T and (need_dy or need_dweights):
-        with _on(dev):
-            st = _lib.load().fack_moe_combine_bwd(
-                dout.data_ptr(), DTYPES[dout.dtype], _ld(dout), y.data_ptr() if need_dweights else None,
-                _ld(y) if need_dweights else 0, w.data_ptr(), T, topk, D, plan.row_of.data_ptr(),
-                plan.offsets.data_ptr(), E, dy.data_ptr() if need_dy else None, D,
-                dw.data_ptr() if need_dweights else None, _stream_handle(dev))
-        _lib.check(st, "fack_moe_combine_bwd")
-    return dy, dw
+    return _combine_grads(dout, y, w, plan.row_of, plan.offsets, need_dy, need_dweights)
 
 
 def _grad_rows(g: torch.Tensor) -> torch.Tensor:
@@ -211,30 +216,30 @@ def _grad_rows(g: torch.Tensor) -> torch.Tensor:
 class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, row_of, src, offsets):
-        plan = MoePlan(row_of, src, offsets)
-        ctx.save_for_backward(*plan)
-        return _gather(x, plan)
+        y = _gather(x, MoePlan(row_of, src, offsets))
+        ctx.save_for_backward(row_of)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        return moe_gather_backward(_grad_rows(dy), MoePlan(*ctx.saved_tensors)), None, None, None
+        return _sum_rows(_grad_rows(dy), None, ctx.saved_tensors[0]), None, None, None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, row_of, src, offsets):
         plan = MoePlan(row_of, src, offsets)
-        need_dw = ctx.needs_input_grad[1]
-        ctx.save_for_backward(y if need_dw else None, weights, *plan)
-        return _combine(y, weights, plan)
+        T, topk = _check_sorted(y, plan)
+        w = _check_weights(weights, T, topk, y.device)
+        ctx.save_for_backward(y if ctx.needs_input_grad[1] else None, w, row_of, offsets)
+        return _sum_rows(y, w, row_of)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        y, weights, *plan = ctx.saved_tensors
-        dy, dw = moe_combine_backward(_grad_rows(dout), y, weights, MoePlan(*plan), ctx.needs_input_grad[0],
-                                      ctx.needs_input_grad[1])
+        y, w, row_of, offsets = ctx.saved_tensors
+        dy, dw = _combine_grads(_grad_rows(dout), y, w, row_of, offsets, *ctx.needs_input_grad[:2])
         return dy, dw, None, None, None
 
 
@@ -277,12 +282,9 @@ def moe_gather_quant(x: torch.Tensor, plan: MoePlan):
         raise ValueError(f"x has {x.shape[0]} rows, the plan {T} tokens")
     if K % BLOCK:
         raise ValueError("K must be a multiple of 128")
-    xq = torch.empty((T * topk, K), dtype=FP8, device=dev)
-    xs = torch.empty((T * topk, K // BLOCK), dtype=torch.float32, device=dev)
+    xq = x.new_empty((T * topk, K), dtype=FP8)
+    xs = x.new_empty((T * topk, K // BLOCK), dtype=torch.float32)
     if T:
-        with _on(dev):
-            st = _lib.load().fack_moe_gather_quant(x.data_ptr(), DTYPES[x.dtype], _ld(x), T, topk, K,
-                                                   plan.row_of.data_ptr(), plan.offsets.data_ptr(), E, xq.data_ptr(),
-                                                   K, xs.data_ptr(), K // BLOCK, _stream_handle(dev))
-        _lib.check(st, "fack_moe_gather_quant")
+        _call("fack_moe_gather_quant", dev, x.data_ptr(), DTYPES[x.dtype], _ld(x), T, topk, K, plan.row_of.data_ptr(),
+              plan.offsets.data_ptr(), E, xq.data_ptr(), K, xs.data_ptr(), K // BLOCK)
     return xq, xs

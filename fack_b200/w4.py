@@ -16,8 +16,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .moe import DTYPES, MoePlan, _check_plan, _check_rows, _ld, _on
-from .ops import _stream_handle
+from .moe import DTYPES, MoePlan, _call, _check_plan, _check_rows, _ld
 
 TYPES = (torch.bfloat16, torch.float16)
 
@@ -51,7 +50,7 @@ def _check_weight(x, w, scales, zeros, lead: tuple):
 
 def _check_out(out, rows: int, N: int, x):
     if out is None:
-        return torch.empty((rows, N), dtype=x.dtype, device=x.device)
+        return x.new_empty((rows, N))
     if not isinstance(out, torch.Tensor) or out.dtype != x.dtype or tuple(out.shape) != (rows, N) or out.stride(1) != 1 \
             or out.device != x.device or (rows > 1 and out.stride(0) < N):
         raise ValueError(f"out must be a {x.dtype} [{rows}, {N}] tensor with unit column stride on {x.device}")
@@ -69,11 +68,8 @@ def gemv_w4(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, zeros: Optio
     M = x.shape[0]
     out = _check_out(out, M, N, x)
     if M:
-        with _on(x.device):
-            st = _lib.load().fack_gemv_w4(x.data_ptr(), DTYPES[x.dtype], _ld(x), w.data_ptr(), scales.data_ptr(),
-                                          DTYPES[scales.dtype], None if zeros is None else zeros.data_ptr(), G,
-                                          out.data_ptr(), _ld(out), M, N, K, _stream_handle(x.device))
-        _lib.check(st, "fack_gemv_w4")
+        _call("fack_gemv_w4", x.device, x.data_ptr(), DTYPES[x.dtype], _ld(x), w.data_ptr(), scales.data_ptr(),
+              DTYPES[scales.dtype], None if zeros is None else zeros.data_ptr(), G, out.data_ptr(), _ld(out), M, N, K)
     return out
 
 
@@ -94,10 +90,8 @@ def gemv_w4_experts(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, plan
                          f"(sorted_rows={bool(sorted_rows)})")
     out = _check_out(out, T * topk, N, x)
     if T:
-        with _on(x.device):
-            st = _lib.load().fack_gemv_w4_experts(
-                x.data_ptr(), DTYPES[x.dtype], _ld(x), w.data_ptr(), scales.data_ptr(), DTYPES[scales.dtype],
-                None if zeros is None else zeros.data_ptr(), G, None if sorted_rows else plan.src.data_ptr(),
-                plan.offsets.data_ptr(), T, topk, E, out.data_ptr(), _ld(out), N, K, _stream_handle(x.device))
-        _lib.check(st, "fack_gemv_w4_experts")
+        _call("fack_gemv_w4_experts", x.device, x.data_ptr(), DTYPES[x.dtype], _ld(x), w.data_ptr(), scales.data_ptr(),
+              DTYPES[scales.dtype], None if zeros is None else zeros.data_ptr(), G,
+              None if sorted_rows else plan.src.data_ptr(), plan.offsets.data_ptr(), T, topk, E, out.data_ptr(),
+              _ld(out), N, K)
     return out
