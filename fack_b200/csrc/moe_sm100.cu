@@ -113,18 +113,27 @@ __global__ void __launch_bounds__(1024) sort_place_kernel(const I* __restrict__ 
 
   int routed = 0;
   if (hist != nullptr) {
-    int before = 0, total = 0;
-    if (e0 < E) {
+    // all blocks' counts, and those of the blocks before this one: the threads
+    // share out the blocks, blockDim / E of them at a time
+    int* all = reinterpret_cast<int*>(sort_smem + E + 1);              // [2][E] in the place of cnt
+    for (int i = threadIdx.x; i < 2 * E; i += blockDim.x) all[i] = 0;
+    __syncthreads();
+    const int at_once = blockDim.x / E, mine_e = threadIdx.x % E;
+    if (static_cast<int>(threadIdx.x) < at_once * E) {
+      int before = 0, total = 0;
 #pragma unroll 8
-      for (int b = 0; b < static_cast<int>(gridDim.x); ++b) {
-        const int c = hist[static_cast<int64_t>(b) * E + e0];
+      for (int b = threadIdx.x / E; b < static_cast<int>(gridDim.x); b += at_once) {
+        const int c = hist[static_cast<int64_t>(b) * E + mine_e];
         before += b < static_cast<int>(blockIdx.x) ? c : 0;
         total += c;
       }
+      atomicAdd(&all[mine_e], total);
+      atomicAdd(&all[E + mine_e], before);
     }
-    const int first = block_scan(total, part, &routed);
+    __syncthreads();
+    const int first = block_scan(e0 < E ? all[e0] : 0, part, &routed);
     if (e0 < E) {
-      base[e0] = first + before;
+      base[e0] = first + all[E + e0];
       if (blockIdx.x == 0) offsets[e0] = first;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) offsets[E] = routed;
