@@ -63,6 +63,7 @@ struct Args {
   int rows, topk, N, K, G, E;
   int tile;                                    // tokens per tile (<= 8 NT)
   int split;                                   // slices of K among a CTA's warps: 1, 2, 4 or 8
+  int groups;                                  // 16-row groups of an item: more than (R - 1) share, at most R share
   int stages;
   int scale_f32;
   unsigned int* status;
@@ -174,14 +175,14 @@ __device__ __forceinline__ float scale_of(uint32_t bits, __half*) {
   return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
 }
 
-// A CTA's item is 16R * share output rows (share = 8 / split) and a tile of
-// tokens; a stage of its ring holds `split` consecutive K blocks of them, one for
-// each slice.  Warp (part, slice) multiplies rows 16R * part .. of block `slice`.
+// A CTA's item is `groups` 16-row groups of the output, dealt out evenly to its
+// share = 8 / split row parts, R or R - 1 to each, and a tile of tokens; a stage of
+// its ring holds `split` consecutive K blocks of them, one for each slice.  Warp
+// (part, slice) multiplies its groups of block `slice`.
 //   weights: per slice, rows of 64 bytes in the 64-byte swizzle (16-byte chunk c of
-//     row r at c ^ (r/2 & 3));
+//     row r at c ^ (r/2 & 3)), in boxes of at most 256 rows;
 //   tokens: rows of split * 256 bytes and a pad;
-//   scales and zero points: per box of at most 256 output rows, a row for each
-//     group of the stage's blocks.
+//   scales and zero points: per box, a row for each group of the stage's blocks.
 // How the chunks are read: a step j of the MMA takes 8 consecutive codes (one
 // word) a lane and row.  With groups of 64 or 128 k a lane's two words may be
 // consecutive, one 8-byte read (WV = 2), else one (WV = 1), since a step may not mix
@@ -195,17 +196,19 @@ struct Stage {
   static constexpr int kWeightBytes = kWarps * kRows * 64;
   static constexpr int kPad = kWords == 1 ? 64 : 16;
   __host__ __device__ static int up(int v, int to) { return (v + to - 1) / to * to; }
-  __host__ __device__ static int box_rows(int split) { return kRows * (kWarps / split) < 256 ? kRows * (kWarps / split) : 256; }
-  __host__ __device__ static int boxes(int split) { return kRows * (kWarps / split) / box_rows(split); }
+  __host__ __device__ static int boxes(int groups) { return groups > 16 ? 2 : 1; }
+  __host__ __device__ static int box_rows(int groups) { return 16 * (groups / boxes(groups)); }
   __host__ __device__ static int x_pitch(int split) { return split * 256 + kPad; }
   __host__ __device__ static int scale_at(int tile, int split) { return up(kWeightBytes + tile * x_pitch(split), 128); }
-  __host__ __device__ static int scale_box(int split, int es) { return up(split * kGroups * box_rows(split) * es, 128); }
-  __host__ __device__ static int zero_at(int tile, int split, int es) {
-    return scale_at(tile, split) + boxes(split) * scale_box(split, es);
+  __host__ __device__ static int scale_box(int split, int groups, int es) {
+    return up(split * kGroups * box_rows(groups) * es, 128);
   }
-  __host__ __device__ static int zero_box(int split) { return up(split * kGroups * box_rows(split), 128); }
-  __host__ __device__ static int bytes(int tile, int split, int es, bool zeros) {
-    return up(zero_at(tile, split, es) + (zeros ? boxes(split) * zero_box(split) : 0), 1024);
+  __host__ __device__ static int zero_at(int tile, int split, int groups, int es) {
+    return scale_at(tile, split) + boxes(groups) * scale_box(split, groups, es);
+  }
+  __host__ __device__ static int zero_box(int split, int groups) { return up(split * kGroups * box_rows(groups), 128); }
+  __host__ __device__ static int bytes(int tile, int split, int groups, int es, bool zeros) {
+    return up(zero_at(tile, split, groups, es) + (zeros ? boxes(groups) * zero_box(split, groups) : 0), 1024);
   }
 };
 template <int R, int NT>
@@ -231,12 +234,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
   __shared__ int abort_flag_s, routed_s;         // rows of an expert: the rest are zeros
   volatile int* abort_flag = &abort_flag_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const int split = p.split, share = kWarps / split, item_rows = kRows * share;
+  const int split = p.split, share = kWarps / split, item_rows = 16 * p.groups;
   const int es = p.scale_f32 ? 4 : 2;
-  const int box_rows = S::box_rows(split), boxes = S::boxes(split), x_pitch = S::x_pitch(split);
-  const int stage_bytes = S::bytes(p.tile, split, es, ZP);
-  const int scale_at = S::scale_at(p.tile, split), scale_box = S::scale_box(split, es);
-  const int zero_at = S::zero_at(p.tile, split, es), zero_box = S::zero_box(split);
+  const int box_rows = S::box_rows(p.groups), boxes = S::boxes(p.groups), x_pitch = S::x_pitch(split);
+  const int stage_bytes = S::bytes(p.tile, split, p.groups, es, ZP);
+  const int scale_at = S::scale_at(p.tile, split), scale_box = S::scale_box(split, p.groups, es);
+  const int zero_at = S::zero_at(p.tile, split, p.groups, es), zero_box = S::zero_box(split, p.groups);
   const uint32_t ring = smem_addr(smem);
   float* red = reinterpret_cast<float*>(smem + p.stages * stage_bytes);
   // the experts that have rows: number, first and last sorted row, running count of token tiles
@@ -415,8 +418,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
     // A wait that gave up leaves the control flow as it is (the barriers below
     // count on every warp) and the status word says that the result is none.
     const int slice = warp % split, part_no = warp / split;
-    const int box = part_no * kRows / box_rows, box_row = part_no * kRows - box * box_rows;
-    const uint32_t w_at = slice * item_rows * 64 + (part_no * kRows + g) * 64 +
+    // this part's groups: R or R - 1 of its box's.  The second box deals them out from
+    // its other end, so that a scheduler's two warps of a CTA have 2 R - 1 together.
+    const int parts = share / boxes, each = box_rows / 16 / parts, more = box_rows / 16 % parts, box = part_no / parts;
+    const int in_box = box ? parts - 1 - part_no % parts : part_no % parts;
+    const int box_row = 16 * (in_box * each + min(in_box, more)), first_row = box * box_rows + box_row;
+    const bool full_part = each + (in_box < more ? 1 : 0) == R;
+    const uint32_t w_at = slice * item_rows * 64 + (first_row + g) * 64 +
                           (((S::kWords == 1 ? 0 : S::kWords == 2 ? q >> 1 : q) ^ ((g >> 1) & 3)) << 4) +
                           (S::kWords == 1 ? q * 4 : S::kWords == 2 ? (q & 1) * 8 : 0);
     // lanes whose token the tile does not have read another's: their columns are not stored
@@ -449,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
           float d[R][NT][4];
           uint32_t mz[R][2];                    // minus the zero points of rows g, g + 8
           uint32_t wl[R][S::kWords], wh[R][S::kWords];   // their words
-#pragma unroll (FL < 128 && R == 4 && NT == 1 && ZP ? FL / 32 : 4)
+#pragma unroll (R == 4 && NT == 1 && (FL == 32 || (FL == 64 && ZP)) ? FL / 32 : 4)
           for (int j = 0; j < 4; ++j) {         // 32 k each
             const bool first = j * 32 % FL == 0;
             if (first) {
@@ -485,6 +493,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
             }
 #pragma unroll
             for (int r = 0; r < R; ++r) {
+              if (r == R - 1 && !full_part) break;
               uint32_t l[4], h[4];
               unpack_codes<T>(wl[r][j % S::kWords], mz[r][0], l);
               unpack_codes<T>(wh[r][j % S::kWords], mz[r][1], h);
@@ -512,6 +521,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
               }
 #pragma unroll
               for (int r = 0; r < R; ++r) {
+                if (r == R - 1 && !full_part) break;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -536,30 +546,32 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int m = 8 * n + 2 * q + (i & 1), row = it.n0 + part_no * kRows + 16 * r + g + (i < 2 ? 0 : 8);
-              if (m < it.count && row < p.N)
+              const int m = 8 * n + 2 * q + (i & 1), row = it.n0 + first_row + 16 * r + g + (i < 2 ? 0 : 8);
+              if (m < it.count && row < p.N && (r < R - 1 || full_part))
                 y[static_cast<int64_t>(m) * p.ldy + row] = C::from(rows_with_x >> m & 1u ? acc[r][n][i] * C::kScale : 0.0f);
             }
       } else {
-        // the slices' partial sums, added in slice order
-        float* mine = red + warp * (kRows * kPitch);
+        // the slices' partial sums [slice][row of the item], added in slice order
+        float* mine = red + (slice * (kRows * share) + first_row + g) * kPitch + 2 * q;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int r = 0; r < R; ++r) {
+          if (r == R - 1 && !full_part) break;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            float* lo = mine + (16 * r + g) * kPitch + 8 * n + 2 * q;
+            float* lo = mine + 16 * r * kPitch + 8 * n;
             float* hi = lo + 8 * kPitch;
             lo[0] = acc[r][n][0];
             lo[1] = acc[r][n][1];
             hi[0] = acc[r][n][2];
             hi[1] = acc[r][n][3];
           }
+        }
         bar_sync(1, kWarps * 32);
         for (int o = threadIdx.x; o < item_rows * it.count; o += kWarps * 32) {
           const int m = o / item_rows, row = o - m * item_rows;
-          const float* f = red + ((row / kRows) * split * kRows + row % kRows) * kPitch + m;
+          const float* f = red + row * kPitch + m;
           float v = 0.0f;
-          for (int w = 0; w < split; ++w) v += f[w * (kRows * kPitch)];
+          for (int w = 0; w < split; ++w) v += f[w * (kRows * share * kPitch)];
           if (it.n0 + row < p.N)
             y[static_cast<int64_t>(m) * p.ldy + it.n0 + row] = C::from(rows_with_x >> m & 1u ? v * C::kScale : 0.0f);
         }
@@ -580,9 +592,10 @@ constexpr int kMaxDevices = 64;
 constexpr int kSmemMost = 226 * 1024, kSmemPair = 112 * 1024;   // a CTA alone on its SM, or one of two
 static std::mutex g_mu;
 
-// A plan: rows of a warp (16R), slices of K, and what it is thought to take.
+// A plan: 16-row groups of a warp (R, or one fewer), slices of K, groups of an item,
+// and what it is thought to take.
 struct Plan {
-  int R, split;
+  int R, split, groups;
   double us;
 };
 
@@ -594,20 +607,33 @@ struct Plan {
 // with two or four, 0.3 with one.  (65536 x 7168, one token: R = 4 with two slices
 // 58 us, R = 2 with one 63; 7168 x 2048: R = 2 with eight slices 11.2, R = 4 12.3;
 // 8192 x 7168, 16 tokens: R = 4 22, R = 2 29.)
-static Plan plan(int NT, double tiles, int N, int K, int sms) {
-  Plan best = {2, kWarps, 1e30};
+// Items need not be full: N = 65536 makes 256 items of 256 rows, two on 108 SMs and
+// one on 40, but 293 of 224 rows, two on nearly all.
+// Where the number of tiles is a guess (`about`), a last round is on average half
+// empty whatever the sizes.
+static double rounds(double items, int at_once, bool about) {
+  const double r = items / at_once;
+  return !about ? ceil(r) : r < 0.8 ? 1.0 : r + 0.6;
+}
+static Plan plan(int NT, double tiles, bool about, int N, int K, int G, int sms) {
+  Plan best = {2, kWarps, 2, 1e30};
   const int KB = (K + kBlkK - 1) / kBlkK;
   for (int R = 2; R <= 4; R += 2) {
     const double step = NT == 1 ? (R == 2 ? 0.56 : 0.95) : (R == 2 ? 0.93 : 1.65);
     const int ctas = NT == 1 ? 2 : 1;
     for (int split = kWarps; split >= 1; split /= 2) {
-      const int rows = 16 * R * (kWarps / split), steps = (KB + split - 1) / split;
-      const double items = tiles * ((N + rows - 1) / rows);
+      const int share = kWarps / split, steps = (KB + split - 1) / split;
       const double join = split == kWarps ? (R == 2 ? 1.0 : 1.7) : split > 1 ? 0.8 : 0.3;
-      const double busy = ceil(items / sms) * (steps * step + join);
-      const double alone = ceil(items / (sms * ctas)) * (0.8 * ctas * steps * step + join);
-      const double us = busy > alone ? busy : alone;
-      if (us < best.us) best = {R, split, us};
+      const int least = G % 128 ? R * share : (R - 1) * share + 1;
+      for (int groups = R * share; groups >= least; --groups) {
+        if (groups > 16 && (groups % 2 || groups / 2 <= (R - 1) * (share / 2))) continue;   // two even boxes
+        const double items = tiles * ((N / 16 + groups - 1) / groups);
+        const double work = steps * step * groups / (R * share);
+        const double busy = rounds(items, sms, about) * (work + join);
+        const double alone = rounds(items, sms * ctas, about) * (0.8 * ctas * work + join);
+        const double us = busy > alone ? busy : alone;
+        if (us < best.us) best = {R, split, groups, us};
+      }
     }
   }
   return best;
@@ -619,7 +645,7 @@ static int launch(Args& a, int sms, cudaStream_t s) {
   const auto kernel = gemv_w4_kernel<T, R, NT, FL, ZP>;
   const int es = a.scale_f32 ? 4 : 2;
   const int room = a.offsets ? (a.E < a.rows ? a.E : a.rows) : 1;
-  const int stage = S::bytes(a.tile, a.split, es, ZP);
+  const int stage = S::bytes(a.tile, a.split, a.groups, es, ZP);
   const int rest = Sums<R, NT>::bytes(a.split) + (4 * room + 1) * static_cast<int>(sizeof(int));
   const bool pair = NT == 1 && rest + 2 * stage <= kSmemPair;
   a.stages = ((pair ? kSmemPair : kSmemMost) - rest) / stage;
@@ -642,18 +668,18 @@ static int launch(Args& a, int sms, cudaStream_t s) {
     }
     per_sm = last[dev][1];
   }
-  const int64_t rows = S::kRows * (kWarps / a.split), ntiles = (a.N + rows - 1) / rows, slots = static_cast<int64_t>(sms) * per_sm;
+  const int64_t rows = 16 * a.groups, ntiles = (a.N + rows - 1) / rows, slots = static_cast<int64_t>(sms) * per_sm;
   // at most this many items: every expert with rows starts one token tile, every a.tile rows fill one
   const int64_t most = (a.rows / a.tile + static_cast<int64_t>(room) + 1) * ntiles;
   if (most > INT32_MAX - slots) return FACK_ERR_BAD_SHAPE;
   CUtensorMap wm, sm, zm;
   const uint64_t E = a.E, N = a.N, K = a.K, groups = a.K / a.G;
-  int st = encode_elems_2d(&wm, a.w, 1, K / 2, E * N, K / 2, kBlkK / 2, S::box_rows(a.split), true);
+  int st = encode_elems_2d(&wm, a.w, 1, K / 2, E * N, K / 2, kBlkK / 2, S::box_rows(a.groups), true);
   if (st == FACK_OK)
-    st = encode_elems_2d(&sm, a.scales, es, N, E * groups, N * es, S::box_rows(a.split), a.split * S::kGroups, false);
+    st = encode_elems_2d(&sm, a.scales, es, N, E * groups, N * es, S::box_rows(a.groups), a.split * S::kGroups, false);
   if (st == FACK_OK) {
     if (ZP)
-      st = encode_elems_2d(&zm, a.zeros, 1, N, E * groups, N, S::box_rows(a.split), a.split * S::kGroups, false);
+      st = encode_elems_2d(&zm, a.zeros, 1, N, E * groups, N, S::box_rows(a.groups), a.split * S::kGroups, false);
     else
       zm = sm;                                  // not used
   }
@@ -675,14 +701,15 @@ static int by_group(Args& a, int NT, int R, int sms, cudaStream_t s) {
   return a.G == 64 ? by_plan<T, 64, ZP>(a, NT, R, sms, s) : by_plan<T, 32, ZP>(a, NT, R, sms, s);
 }
 
-// Token tiles that `rows` rows, sent to E experts at random, are expected to take:
-// E times the mean of ceil(x / tile) over a Poisson x.
-static double expected_tiles(int64_t rows, int E, int tile) {
-  const double mean = static_cast<double>(rows) / E;
+// Token tiles that T tokens of topk experts each are expected to take, chosen at
+// random without repeats: E times the mean of ceil(x / tile) over a binomial x.
+static double expected_tiles(int T, int topk, int E, int tile) {
+  const double q = static_cast<double>(topk) / E, mean = q * T;
+  if (q >= 1.0) return static_cast<double>(E) * ((static_cast<int64_t>(T) * topk / E + tile - 1) / tile);
   if (mean > 200.0) return E * (mean / tile + 0.5);
-  double sum = 0.0, p = exp(-mean);
-  for (int x = 1; x < 600; ++x) {
-    p *= mean / x;
+  double sum = 0.0, p = exp(T * log1p(-q));
+  for (int x = 1; x <= T && x < 600; ++x) {
+    p *= static_cast<double>(T - x + 1) / x * q / (1.0 - q);
     sum += p * ((x + tile - 1) / tile);
   }
   return E * sum;
@@ -698,19 +725,20 @@ static void choose(Args& a, int tokens, int sms, int* NT, int* R) {
     double tiles;
     if (a.offsets) {
       tile[i] = tokens < most ? tokens : most;
-      tiles = expected_tiles(a.rows, a.E, tile[i]);
+      tiles = expected_tiles(tokens, a.topk, a.E, tile[i]);
     } else {
       const int64_t n = (static_cast<int64_t>(a.rows) + most - 1) / most;
       tile[i] = static_cast<int>((a.rows + n - 1) / n);      // evenly filled
       tiles = static_cast<double>(n);
     }
-    p[i] = plan(i + 1, tiles, a.N, a.K, sms);
+    p[i] = plan(i + 1, tiles, a.offsets != nullptr, a.N, a.K, a.G, sms);
   }
   const int i = tile[1] > 8 && p[1].us < p[0].us;
   *NT = i + 1;
   *R = p[i].R;
   a.tile = tile[i];
   a.split = p[i].split;
+  a.groups = p[i].groups;
 }
 
 static int run(Args& a, int dtype, int scale_dtype, int tokens, void* stream) {
