@@ -7,24 +7,33 @@
 // G consecutive k, x and y bf16 or fp16.  With a plan of tokens sorted by
 // expert the same for every expert's rows and weights.
 //
-// The call is the weight stream: N*K/2 bytes that are read once.  Everything
-// here serves to keep that stream going:
-//   * A CTA owns 16*R output rows; its 8 warps take the 128-wide K blocks in
-//     turn (warp w the blocks w, w + 8, ...), so at any time the CTA reads 512
-//     contiguous bytes of each row.  CTAs are persistent: each walks a list of
-//     (expert, row tile, token tile) items with one running ring of cp.async
-//     stages per warp, which goes on into the next item while the last one is
-//     summed, and no barrier stands between a warp and its own loads.
+// The call is the weight stream, N*K/2 bytes that are read once: 13 T codes a
+// second at the memory's rate, which leaves a scheduler about 22 cycles for each
+// warp-wide word of 8 codes a lane.  So instructions count as much as bytes:
 //   * The products go to the warp MMA (m16n8k16, fp32 accumulators): 16 weight
-//     rows x 8 tokens.  A code is turned into a 16-bit float of c - z exactly (see
-//     Codes), so the MMA's products are exact and the only roundings are fp32
-//     additions, the fp32 scale per group, and the last one to the output type.
-//   * A word of 8 consecutive codes gives the pairs (i, i + 4) by one shift and
-//     mask each; the tokens are put in the same order (the MMA does not care
-//     which k goes where, if both operands agree).
+//     rows x 8 tokens.  A word of 8 codes becomes four operand registers of the
+//     exact 16-bit floats c - z with one shift, four masks and four fma (see
+//     Codes): every product is exact, and the only roundings are fp32 additions,
+//     the fp32 scale per group and the last one to the output type.
+//   * The pairs (i, i + 4) that a mask picks out of a word are met by the tokens in
+//     the same order (the MMA does not care which k goes where, if both operands
+//     agree).
+//   * One warp of a CTA brings the data (TMA boxes of weights, scales and zero
+//     points, one bulk copy a token) into a ring of stages; eight multiply, each
+//     its own rows of one of `split` slices of K.  CTAs are persistent over a list
+//     of (expert, row tile, token tile) items, and the ring runs on from one item
+//     into the next.  Rows per warp, slices and rows per item follow a cost model
+//     (see plan): few rows are split along K, many are dealt out evenly.
+// Measured on B200, L2 flushed: 65536 x 7168 (235 MB) with one token 55 us = 4.3 TB/s,
+// with eight 58 us, with thirteen 90-98 us; the copies alone take 43-46 us (55-61 with
+// thirteen).  ncu there: 15 instructions a word, 53 % of the issue slots, ALU 45 %,
+// tensor pipe 27 %, DRAM 60 %: bound by the unpacking's latency and issue.
 // The warp MMA, not tcgen05: 8 or 16 tokens fill a fraction of a tcgen05 tile,
 // 4-bit codes with arbitrary scales are no operand type of it, and dequantised
-// tiles would have to pass through shared memory once more.
+// tiles would have to pass through shared memory once more.  Tokens in three 8-bit
+// digits and codes as they are (exact, a third of the unpacking) were measured with
+// the int8 MMA (56 / 71 / 126 us for 1 / 8 / 13 tokens: three times the MMAs and
+// accumulators) and the fp8 MMA (92 us: mma.sync converts its operands here).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -48,7 +57,7 @@ constexpr int kBlkK = 128;                     // k per warp and stage
 constexpr int kMaxStages = 8;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopk = 64;
-constexpr unsigned kStW4 = 128u;               // status flag: a wait in these kernels gave up
+constexpr unsigned kStW4 = 256u;               // status flag: a wait in these kernels gave up
 
 struct Args {
   const void* x;                               // [rows or tokens, K]
@@ -70,13 +79,14 @@ struct Args {
   uint64_t timeout_ns;
 };
 
-// A word's codes 0..7 as four registers of two 16-bit floats each, (c - z) *
-// kUnit exactly, codes i and i + 4 together.  A masked code is a subnormal, c or
+// A word's codes 0..7 as four registers of two 16-bit floats each, exactly
+// (c - z) / kScale, codes i and i + 4 together.  A masked code is a subnormal, c or
 // 16c units of the type's smallest (in bf16 the top bit of 16c is the exponent's
 // lowest, where the normal numbers go on at the same spacing), and one fused
 // multiply-add scales it and takes the zero point away: 1 shift, 4 masks, 4 fma
-// for 8 codes.  The ALU, which has half the rate of the fma pipe, does the rest
-// of the address work too and is what the kernel ran out of with more shifts.
+// for 8 codes.  Or-ing the code into 128 or 1024 and subtracting takes 3 shifts;
+// shifts and masks run at half the rate of the fma (95 -> 74 us for 16 rows of
+// 4096 x 7168 in an earlier form of the kernel).
 template <typename T> struct Codes;
 template <> struct Codes<__nv_bfloat16> {
   using T2 = __nv_bfloat162;
@@ -151,9 +161,6 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
 __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[1]) { v[0] = lds32(a); }
 __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[2]) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a));
-}
-__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[4]) {
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a));
 }
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
@@ -425,8 +432,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
     const int box_row = 16 * (in_box * each + min(in_box, more)), first_row = box * box_rows + box_row;
     const bool full_part = each + (in_box < more ? 1 : 0) == R;
     const uint32_t w_at = slice * item_rows * 64 + (first_row + g) * 64 +
-                          (((S::kWords == 1 ? 0 : S::kWords == 2 ? q >> 1 : q) ^ ((g >> 1) & 3)) << 4) +
-                          (S::kWords == 1 ? q * 4 : S::kWords == 2 ? (q & 1) * 8 : 0);
+                          (((S::kWords == 1 ? 0 : q >> 1) ^ ((g >> 1) & 3)) << 4) + (S::kWords == 1 ? q * 4 : (q & 1) * 8);
     // lanes whose token the tile does not have read another's: their columns are not stored
     uint32_t x_at[NT];
 #pragma unroll
@@ -484,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
             }
             if (j % S::kWords == 0) {
               // part j / WV: 16 bytes on (WV = 1), 32 bytes on (WV = 2)
-              const uint32_t wj = (st + w_at) ^ (S::kWords == 1 ? j << 4 : S::kWords == 2 ? (j >> 1) << 5 : 0);
+              const uint32_t wj = (st + w_at) ^ (S::kWords == 1 ? j << 4 : (j >> 1) << 5);
 #pragma unroll
               for (int r = 0; r < R; ++r) {
                 lds_words(wj + r * 1024, wl[r]);
@@ -599,22 +605,25 @@ struct Plan {
   double us;
 };
 
-// The cheapest R and split for `tiles` token tiles of up to 8 NT tokens.  Measured
-// on B200, microseconds: a step of an item (one K block a warp) costs an SM 0.56
-// (R = 2) or 0.95 (R = 4) with 8 tokens and two CTAs on it, 0.93 or 1.65 with 16 and one
-// CTA; one CTA of two alone takes 1.6 times as long for its own;
-// joining the slices of an item costs 1.0 (R = 2) or 1.7 (R = 4) with eight, 0.8
-// with two or four, 0.3 with one.  (65536 x 7168, one token: R = 4 with two slices
-// 58 us, R = 2 with one 63; 7168 x 2048: R = 2 with eight slices 11.2, R = 4 12.3;
-// 8192 x 7168, 16 tokens: R = 4 22, R = 2 29.)
-// Items need not be full: N = 65536 makes 256 items of 256 rows, two on 108 SMs and
-// one on 40, but 293 of 224 rows, two on nearly all.
-// Where the number of tiles is a guess (`about`), a last round is on average half
-// empty whatever the sizes.
+// Rounds of `items` over `at_once` places.  Where the number of items is a guess
+// (`about`), a last round is on average half empty whatever the sizes.
 static double rounds(double items, int at_once, bool about) {
   const double r = items / at_once;
   return !about ? ceil(r) : r < 0.8 ? 1.0 : r + 0.6;
 }
+
+// The cheapest R, split and item for `tiles` token tiles of up to 8 NT tokens.
+// Measured on B200, in microseconds: a step of an item (one K block a warp) costs an
+// SM 0.56 (R = 2) or 0.95 (R = 4) with 8 tokens and two CTAs on it, 0.93 or 1.65 with
+// 16 tokens and one CTA; one CTA of two, alone on its SM, takes 0.8 of two; joining the
+// slices of an item costs 1.0 (R = 2) or 1.7 (R = 4) with eight, 0.8 with two or four,
+// 0.3 with one.  (65536 x 7168, one token: R = 4 with two slices 58 us, R = 2 with one
+// 68; 7168 x 2048: R = 2 with eight slices 10-11, R = 4 12; 8192 x 7168, 16 tokens:
+// R = 4 22, R = 2 29.)
+// Items need not be full: N = 65536 makes 256 items of 256 rows, two on 108 SMs and
+// one on 40, but 293 of 224 rows, two on nearly all (58 -> 55 us).  With groups below
+// 128 the branch around a warp's last rows costs more than that (137 -> 172 us for 64
+// experts of 7168 x 2048), so there they stay full.
 static Plan plan(int NT, double tiles, bool about, int N, int K, int G, int sms) {
   Plan best = {2, kWarps, 2, 1e30};
   const int KB = (K + kBlkK - 1) / kBlkK;

@@ -64,6 +64,8 @@ def _call(name: str, dev: torch.device, *args) -> None:
 
 def _check_plan(plan, dev: torch.device):
     """(T, k, E) of a plan on ``dev``."""
+    if not isinstance(plan, MoePlan):
+        raise ValueError("plan must be the MoePlan of moe_sort")
     row_of, src, offsets = plan
     for name, t, dim in (("row_of", row_of, 2), ("src", src, 1), ("offsets", offsets, 1)):
         if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dim or t.device != dev \
@@ -213,6 +215,15 @@ def _grad_rows(g: torch.Tensor) -> torch.Tensor:
     return g if g.shape[1] == 1 or g.stride(1) == 1 else g.contiguous()
 
 
+def _refuse_captured_leaf(*inputs) -> None:
+    """No gradient of a leaf inside a CUDA-graph capture: where an eager graph of
+    the same leaf is alive, autograd would make the capture wait on that graph's
+    stream, which ends the process.  The backward functions have no such state."""
+    if torch.cuda.is_current_stream_capturing() and any(t.requires_grad and t.is_leaf for t in inputs):
+        raise ValueError("a captured gather or combine takes no leaf that requires grad; call moe_gather_backward / "
+                         "moe_combine_backward in the capture instead, or detach the input")
+
+
 class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, row_of, src, offsets):
@@ -246,8 +257,10 @@ class _Combine(torch.autograd.Function):
 def moe_gather(x: torch.Tensor, plan: MoePlan) -> torch.Tensor:
     """The tokens' rows in expert order: y [T*k, D] with y[r] = x[src[r] // k],
     zeros where a row has no pair.  ``x`` [T, D] fp32, bf16 or fp16, any row
-    stride.  Differentiable in x (:func:`moe_gather_backward`)."""
-    if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
+    stride.  Differentiable in x (:func:`moe_gather_backward`); inside a CUDA-graph
+    capture x may not be a leaf that requires grad."""
+    if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled() and isinstance(plan, MoePlan):
+        _refuse_captured_leaf(x)
         return _Gather.apply(x, *plan)
     return _gather(x, plan)
 
@@ -257,10 +270,14 @@ def moe_combine(y: torch.Tensor, weights: torch.Tensor, plan: MoePlan) -> torch.
     y[row_of[t, j]] over the pairs that have a row, in fp32, slots in order,
     rounded once to y's type.  ``y`` [T*k, D] fp32, bf16 or fp16, any row
     stride; ``weights`` fp32 [T, k].  Differentiable in both
-    (:func:`moe_combine_backward`)."""
+    (:func:`moe_combine_backward`); inside a CUDA-graph capture neither may be a
+    leaf that requires grad."""
     if weights is None:
         raise ValueError("weights must be a float32 [T, k] tensor")
-    if torch.is_grad_enabled() and (getattr(y, "requires_grad", False) or getattr(weights, "requires_grad", False)):
+    if torch.is_grad_enabled() and isinstance(plan, MoePlan) and (getattr(y, "requires_grad", False)
+                                                                  or getattr(weights, "requires_grad", False)):
+        if isinstance(y, torch.Tensor) and isinstance(weights, torch.Tensor):
+            _refuse_captured_leaf(y, weights)
         return _Combine.apply(y, weights, *plan)
     return _combine(y, weights, plan)
 

@@ -354,6 +354,41 @@ def test_two_captured_graphs_and_another_stream(cuda_device):
                 assert torch.equal(a, b)
 
 
+def test_gradients_inside_a_capture(cuda_device):
+    """A captured pass may differentiate what it computes; a leaf is refused (before
+    anything is recorded), the backward functions are the way for one."""
+    T, k, E, D = 50, 3, 8, 96
+    plan = gpu_plan(T, k, E, 2, cuda_device)
+    x, w, dout = torch.randn((T, D), device=cuda_device), torch.rand((T, k), device=cuda_device), torch.randn((T, D), device=cuda_device)
+
+    def step(a, b):
+        y = fb.moe_gather(a * 2, plan)
+        out = fb.moe_combine(y, b * 0.5, plan)
+        return [out, *torch.autograd.grad(out, (a, b), dout)]
+
+    ref = step(x.clone().requires_grad_(), w.clone().requires_grad_())
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(a, b)
+    graph.replay()
+    torch.cuda.synchronize()
+    for g, r in zip(got, ref):
+        assert torch.equal(g, r)
+    y = fb.moe_gather(x, plan)
+    other = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(other):
+        for f in (lambda: fb.moe_gather(a, plan), lambda: fb.moe_combine(y, b, plan),
+                  lambda: fb.moe_combine(y.detach().requires_grad_(), w, plan)):
+            with pytest.raises(ValueError):
+                f()
+        dx = fb.moe_gather_backward(y, plan)
+    other.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(dx, fb.moe_gather_backward(y, plan))
+
+
 def test_rows_beyond_32_bit_offsets(cuda_device):
     """Sorted rows past 2^31 elements: the last rows land where they belong."""
     T, k, D = 40000, 8, 7168                       # 2.3e9 elements of y

@@ -102,6 +102,6 @@ def test_plan_checks():
     assert moe._check_plan(plan, cpu) == (4, 2, 3)
     for bad in (plan._replace(row_of=plan.row_of.long()), plan._replace(src=plan.src[:7]),
                 plan._replace(offsets=plan.offsets[:1]), plan._replace(row_of=plan.row_of.t()),
-                plan._replace(row_of=plan.row_of.reshape(-1)), plan._replace(offsets=None)):
+                plan._replace(row_of=plan.row_of.reshape(-1)), plan._replace(offsets=None), tuple(plan), None):
         with pytest.raises(ValueError):
             moe._check_plan(bad, cpu)

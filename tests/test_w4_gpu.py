@@ -267,3 +267,92 @@ def test_a_routed_layer_and_its_graph(cuda_device):
             eager = routed_layer(*to(cuda_device, *sets[2]), *dev, E)[0]
         torch.cuda.synchronize()
         assert torch.equal(out, runs[i]) and torch.equal(eager, runs[2])
+
+
+FIRST_CALLS = """
+import torch
+import fack_b200 as fb
+d = torch.device("cuda", 0)
+T, k, E = 700, 4, 6                                   # several sort blocks
+ids = torch.arange(T * k, device=d).reshape(T, k) % E
+x = torch.randn((T, 256), device=d).bfloat16()
+w = torch.randint(0, 256, (E, 64, 128), dtype=torch.uint8, device=d)
+s = torch.rand((E, 4, 64), device=d)
+gates = torch.rand((T, k), device=d)
+
+def step():
+    plan = fb.moe_sort(ids, E)
+    xq, xs = fb.moe_gather_quant(x, plan)
+    y = fb.gemv_w4_experts(x, w, s, plan)
+    out = fb.moe_combine(y, gates, plan)
+    dy, dw = fb.moe_combine_backward(out, y, gates, plan)
+    return [*plan, xq.view(torch.uint8), xs, y, out, dy, dw, fb.moe_gather_backward(fb.moe_gather(x, plan), plan),
+            fb.gemv_w4(x[:3], w[0], s[0])]
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):                         # nothing of the library has run before
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in got]
+assert all(torch.equal(a, b) for a, b in zip(got, step())) and fb.device_status() == 0
+print("captured first")
+"""
+
+
+def test_a_process_whose_first_calls_are_captured(cuda_device):
+    import subprocess
+    import sys
+    from pathlib import Path
+    run = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=Path(__file__).resolve().parents[1], capture_output=True,
+                         text=True, timeout=300)
+    assert run.returncode == 0 and "captured first" in run.stdout, run.stdout + run.stderr
+
+
+def test_calls_from_two_threads(cuda_device):
+    """The C entries' own state (kernel attributes, plans) under concurrent first and later calls."""
+    import threading
+    g = torch.Generator().manual_seed(5)
+    cases = []
+    for i, (M, N, K, G) in enumerate([(1, 48, 256, 64), (9, 96, 512, 128), (3, 32, 160, 32), (16, 64, 1024, 256)]):
+        w, s, z = weight((), N, K, G, i % 2 == 1, torch.float32, i, exact=True)
+        x = few_ones(M, K, i, torch.float16)
+        cases.append((to(cuda_device, x, w, s, z), orc.product_ref(x, w, s, z)[0]))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(first):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for i in range(60):
+                args, ref = cases[(first + i) % len(cases)]
+                y = fb.gemv_w4(*args)
+                if not torch.equal(y.cpu().double(), ref):
+                    wrong.append((first, i))
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong and fb.device_status() == 0
+
+
+@pytest.mark.parametrize("M", [1, 13, 40])
+@pytest.mark.parametrize("N,K,G", [(16 * 37, 128 * 9, 128), (16 * 293, 128 * 2, 256), (4096 + 16, 96, 32), (16 * 600, 64, 64),
+                                   (16 * 1031, 128, 128)])
+def test_exact_over_the_plans(cuda_device, M, N, K, G):
+    """Row counts that leave items, parts of items and the last box of an item partly filled."""
+    w, s, z = weight((), N, K, G, M == 13, torch.bfloat16, N + K, exact=True)
+    x = few_ones(M, K, N, torch.bfloat16)
+    assert torch.equal(fb.gemv_w4(*to(cuda_device, x, w, s, z)).cpu().double(), orc.product_ref(x, w, s, z)[0])
+
+
+def test_a_stack_of_most_experts(cuda_device):
+    """1024 experts, a few of which have rows: the first, the last and neighbours."""
+    E, N, K = 1024, 32, 64
+    w, s, _ = weight((E,), N, K, 32, False, torch.float32, 1, exact=True)
+    ids = torch.tensor([[0, 1023], [511, 512], [1023, 1023], [7, -1], [1024, 0]])
+    plan = fb.moe_sort(ids.to(cuda_device), E)
+    x = few_ones(5, K, 2, torch.float16)
+    row_of, src, offsets = moe_orc.sort_ref(ids, E)
+    ref = orc.experts_ref(moe_orc.gather_ref(x, src, 2), w, s, None, offsets, 10)[0]
+    assert torch.equal(fb.gemv_w4_experts(*to(cuda_device, x, w, s), plan).cpu().double(), ref)
