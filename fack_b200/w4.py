@@ -21,29 +21,31 @@ from .moe import DTYPES, MoePlan, _call, _check_plan, _check_rows, _ld
 TYPES = (torch.bfloat16, torch.float16)
 
 
+def _part(name: str, t, types: tuple, lead: tuple, dev) -> None:
+    dims = len(lead) + 2
+    if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype not in types or t.dim() != dims \
+            or (lead and t.shape[0] != lead[0]) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dims}-D tensor of {' or '.join(str(d) for d in types)} on {dev}"
+                         + (f" with {lead[0]} experts" if lead else ""))
+
+
 def _check_weight(x, w, scales, zeros, lead: tuple):
     """(N, K, G) of a 4-bit weight with leading dimensions ``lead`` for x [*, K]."""
     K, dev = x.shape[1], x.device
-    dims = len(lead) + 2
-    for name, t, types in (("w", w, (torch.uint8,)), ("scales", scales, (torch.float32, x.dtype)),
-                           ("zeros", zeros, (torch.uint8,))):
-        if t is None and name == "zeros":
-            continue
-        if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype not in types or t.dim() != dims \
-                or tuple(t.shape[:-2]) != lead or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous {dims}-D tensor of {' or '.join(str(d) for d in types)} on {dev}"
-                             + (f" with {lead[0]} experts" if lead else ""))
+    _part("w", w, (torch.uint8,), lead, dev)
+    _part("scales", scales, (torch.float32, x.dtype), lead, dev)
+    if zeros is not None:
+        _part("zeros", zeros, (torch.uint8,), lead, dev)
     N, half = w.shape[-2:]
-    groups = scales.shape[-2]
-    if half * 2 != K or scales.shape[-1] != N or groups < 1 or K % groups or \
-            (zeros is not None and zeros.shape != scales.shape):
+    groups, width = scales.shape[-2:]
+    if half * 2 != K or width != N or groups < 1 or K % groups or (zeros is not None and zeros.shape != scales.shape):
         raise ValueError(f"shape mismatch: x {tuple(x.shape)}, w {tuple(w.shape)}, scales {tuple(scales.shape)}, "
                          f"zeros {None if zeros is None else tuple(zeros.shape)}")
     G = K // groups
-    if N < 16 or N % 16 or (G not in (32, 64) and G % 128):
+    if N < 16 or N % 16 or (G != 32 and G != 64 and G % 128):
         raise ValueError(f"4-bit products need N % 16 == 0 and groups of 32, 64 or a multiple of 128 along K "
                          f"(N = {N}, group = {G})")
-    if torch.is_grad_enabled() and (x.requires_grad or scales.requires_grad):
+    if (x.requires_grad or scales.requires_grad) and torch.is_grad_enabled():
         raise ValueError("4-bit products have no gradient; detach the operands or call under torch.no_grad()")
     return N, K, G
 
