@@ -346,6 +346,14 @@ def test_exact_over_the_plans(cuda_device, M, N, K, G):
     assert torch.equal(fb.gemv_w4(*to(cuda_device, x, w, s, z)).cpu().double(), orc.product_ref(x, w, s, z)[0])
 
 
+def test_the_longest_rows(cuda_device):
+    """K = 2^20, and one token more than fits a tile."""
+    N, K, G = 16, 1 << 20, 4096
+    w, s, _ = weight((), N, K, G, False, torch.float32, 3, exact=True)
+    x = few_ones(9, K, 4, torch.bfloat16)
+    assert torch.equal(fb.gemv_w4(*to(cuda_device, x, w, s)).cpu().double(), orc.product_ref(x, w, s, None)[0])
+
+
 def test_a_stack_of_most_experts(cuda_device):
     """1024 experts, a few of which have rows: the first, the last and neighbours."""
     E, N, K = 1024, 32, 64
