@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(1024) sort_count_kernel(const I* __restrict__ 
 
 // Ranks and scatters each block's share, chunk by chunk.  A warp takes a
 // contiguous run of a chunk, 32 pairs a round: lanes with the same expert find
-// each other with match.any, their rank is the warp's running count plus the
+// each other by a ballot for each bit of its number, their rank is the warp's running count plus the
 // lanes before them, so order is kept without an atomic.  A column scan over
 // the warps then turns counts into rows.  With one block (hist NULL) the counts
 // of the first and only chunk are the histogram.
@@ -110,6 +110,7 @@ __global__ void __launch_bounds__(1024) sort_place_kernel(const I* __restrict__ 
   const int64_t begin = blockIdx.x * share;
   const int64_t end = begin + share < pairs ? begin + share : pairs;
   const int e0 = threadIdx.x;                                        // blockDim >= E
+  const int bits = 32 - __clz(E);                                    // of an expert's number, E itself included
 
   int routed = 0;
   if (hist != nullptr) {
@@ -150,7 +151,12 @@ __global__ void __launch_bounds__(1024) sort_place_kernel(const I* __restrict__ 
     for (int i = 0; i < kSortRounds; ++i) expert[i] = expert_of(ids, w0 + 32 * i, end, E);
 #pragma unroll
     for (int i = 0; i < kSortRounds; ++i) {
-      const unsigned same = __match_any_sync(0xffffffffu, expert[i]);
+      unsigned same = 0xffffffffu;                                   // lanes with this lane's expert
+      for (int bit = 0; bit < bits; ++bit) {
+        const bool set = expert[i] >> bit & 1;
+        const unsigned those = __ballot_sync(0xffffffffu, set);
+        same &= set ? those : ~those;
+      }
       const int ahead = __popc(same & ((1u << lane) - 1u));
       rank[i] = mine[expert[i]] + ahead;
       __syncwarp();
@@ -298,13 +304,15 @@ __global__ void __launch_bounds__(256) gather_kernel(const void* __restrict__ xp
   zero_tail<U>(y, ldy, nvec, rows, *routed, U{});
 }
 
-// out[t] = sum_j w[t, j] * y[row_of[t, j]] (w NULL: 1), fp32, slots in order.
-template <typename T, int V>
+// out[t] = sum_j w[t, j] * y[row_of[t, j]] (w NULL: 1), fp32, slots in order.  A
+// thread has SL slots of U places of the row in flight, eight 16-byte loads
+// whether a token has two experts or eight: with two loads the rows of 16384 x 2
+// experts, 1024 wide bf16, came at 0.60 of the copy rate.
+template <typename T, int V, int SL, int U>
 __global__ void __launch_bounds__(256) combine_kernel(const T* __restrict__ y, int64_t ldy, const float* __restrict__ w,
                                                       int nvec, int topk, int64_t rows, const int* __restrict__ row_of,
                                                       T* __restrict__ out, int64_t ldo) {
   using P = Pack<T, V>;
-  constexpr int kAhead = 8;                       // rows in flight
   __shared__ int at[kMaxTopk];
   __shared__ float gate[kMaxTopk];
   const int64_t t = blockIdx.x;
@@ -314,36 +322,51 @@ __global__ void __launch_bounds__(256) combine_kernel(const T* __restrict__ y, i
     gate[j] = w ? w[t * topk + j] : 1.0f;
   }
   __syncthreads();
-  for (int v = blockIdx.y * blockDim.x + threadIdx.x; v < nvec; v += gridDim.y * blockDim.x) {
-    float acc[V];
+  const int step = gridDim.y * blockDim.x;
+  for (int v0 = blockIdx.y * blockDim.x + threadIdx.x; v0 < nvec; v0 += U * step) {
+    float acc[U][V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-    for (int j0 = 0; j0 < topk; j0 += kAhead) {
-      P p[kAhead];
+    for (int k = 0; k < U; ++k)
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (j0 + u < topk && at[j0 + u] >= 0)
-          p[u] = *reinterpret_cast<const P*>(y + at[j0 + u] * ldy + static_cast<int64_t>(v) * V);
+      for (int i = 0; i < V; ++i) acc[k][i] = 0.0f;
+    for (int j0 = 0; j0 < topk; j0 += SL) {
+      P p[SL][U];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
+      for (int u = 0; u < SL; ++u)
+        if (j0 + u < topk && at[j0 + u] >= 0) {
+          const T* row = y + at[j0 + u] * ldy;
+#pragma unroll
+          for (int k = 0; k < U; ++k)
+            if (v0 + k * step < nvec) p[u][k] = *reinterpret_cast<const P*>(row + static_cast<int64_t>(v0 + k * step) * V);
+        }
+#pragma unroll
+      for (int u = 0; u < SL; ++u)
         if (j0 + u < topk && at[j0 + u] >= 0) {
           const float g = gate[j0 + u];
-          float f[V];
-          unpack(p[u], f);
 #pragma unroll
-          for (int i = 0; i < V; ++i) acc[i] = fmaf(g, f[i], acc[i]);
+          for (int k = 0; k < U; ++k)
+            if (v0 + k * step < nvec) {
+              float f[V];
+              unpack(p[u][k], f);
+#pragma unroll
+              for (int i = 0; i < V; ++i) acc[k][i] = fmaf(g, f[i], acc[k][i]);
+            }
         }
     }
-    P o;
-    pack(o, acc);
-    *reinterpret_cast<P*>(out + t * ldo + static_cast<int64_t>(v) * V) = o;
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (v0 + k * step < nvec) {
+        P o;
+        pack(o, acc[k]);
+        *reinterpret_cast<P*>(out + t * ldo + static_cast<int64_t>(v0 + k * step) * V) = o;
+      }
   }
 }
 
 // dy[row_of[t, j]] = w[t, j] * dout[t] and dw[t, j] = <dout[t], y[row_of[t, j]]>
 // (either may be NULL), one block a token.  The dot products are fp32: each
 // thread's own columns in order, then the lanes, then the warps.
-template <typename T, int V>
+template <typename T, int V, int SL, int U>
 __global__ void __launch_bounds__(256, 3) combine_bwd_kernel(const T* __restrict__ dout, int64_t ldd,
                                                           const T* __restrict__ y, int64_t ldy,
                                                           const float* __restrict__ w, int nvec, int topk, int64_t rows,
@@ -351,10 +374,9 @@ __global__ void __launch_bounds__(256, 3) combine_bwd_kernel(const T* __restrict
                                                           const int* __restrict__ routed, T* __restrict__ dy,
                                                           int64_t lddy, float* __restrict__ dw) {
   using P = Pack<T, V>;
-  constexpr int kAhead = 4;
   __shared__ int at[kMaxTopk];
   __shared__ float gate[kMaxTopk];
-  __shared__ float sums[8][kAhead];
+  __shared__ float sums[8][SL];
   const int64_t t = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   for (int j = threadIdx.x; j < topk; j += blockDim.x) {
@@ -363,52 +385,63 @@ __global__ void __launch_bounds__(256, 3) combine_bwd_kernel(const T* __restrict
     gate[j] = w[t * topk + j];
   }
   __syncthreads();
-  for (int j0 = 0; j0 < topk; j0 += kAhead) {
-    float dot[kAhead];
+  const int step = blockDim.x;
+  for (int j0 = 0; j0 < topk; j0 += SL) {
+    float dot[SL];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) dot[u] = 0.0f;
-    for (int v = threadIdx.x; v < nvec; v += blockDim.x) {
-      const P dp = *reinterpret_cast<const P*>(dout + t * ldd + static_cast<int64_t>(v) * V);
-      float d[V];
-      unpack(dp, d);
-      P p[kAhead];
+    for (int u = 0; u < SL; ++u) dot[u] = 0.0f;
+    for (int v0 = threadIdx.x; v0 < nvec; v0 += U * step) {
+      P dp[U], p[SL][U];
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (v0 + k * step < nvec) dp[k] = *reinterpret_cast<const P*>(dout + t * ldd + static_cast<int64_t>(v0 + k * step) * V);
       if (dw) {
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-          if (j0 + u < topk && at[j0 + u] >= 0)
-            p[u] = *reinterpret_cast<const P*>(y + at[j0 + u] * ldy + static_cast<int64_t>(v) * V);
+        for (int u = 0; u < SL; ++u)
+          if (j0 + u < topk && at[j0 + u] >= 0) {
+            const T* row = y + at[j0 + u] * ldy;
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+              if (v0 + k * step < nvec) p[u][k] = *reinterpret_cast<const P*>(row + static_cast<int64_t>(v0 + k * step) * V);
+          }
       }
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        if (j0 + u >= topk || at[j0 + u] < 0) continue;
-        if (dw) {
-          float f[V];
-          unpack(p[u], f);
+      for (int k = 0; k < U; ++k) {
+        if (v0 + k * step >= nvec) break;
+        float d[V];
+        unpack(dp[k], d);
 #pragma unroll
-          for (int i = 0; i < V; ++i) dot[u] = fmaf(d[i], f[i], dot[u]);
-        }
-        if (dy) {
-          P o;
-          float f[V];
+        for (int u = 0; u < SL; ++u) {
+          if (j0 + u >= topk || at[j0 + u] < 0) continue;
+          if (dw) {
+            float f[V];
+            unpack(p[u][k], f);
 #pragma unroll
-          for (int i = 0; i < V; ++i) f[i] = gate[j0 + u] * d[i];
-          pack(o, f);
-          *reinterpret_cast<P*>(dy + at[j0 + u] * lddy + static_cast<int64_t>(v) * V) = o;
+            for (int i = 0; i < V; ++i) dot[u] = fmaf(d[i], f[i], dot[u]);
+          }
+          if (dy) {
+            P o;
+            float f[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = gate[j0 + u] * d[i];
+            pack(o, f);
+            *reinterpret_cast<P*>(dy + at[j0 + u] * lddy + static_cast<int64_t>(v0 + k * step) * V) = o;
+          }
         }
       }
     }
     if (dw) {
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
+      for (int u = 0; u < SL; ++u) {
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], d);
       }
       if (lane == 0) {
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) sums[warp][u] = dot[u];
+        for (int u = 0; u < SL; ++u) sums[warp][u] = dot[u];
       }
       __syncthreads();
-      if (threadIdx.x < kAhead && j0 + threadIdx.x < topk) {
+      if (threadIdx.x < SL && j0 + threadIdx.x < topk) {
         float s = 0.0f;
         for (int i = 0; i < warps; ++i) s += sums[i][threadIdx.x];
         dw[t * topk + j0 + threadIdx.x] = at[j0 + threadIdx.x] >= 0 ? s : 0.0f;
@@ -588,23 +621,59 @@ static int row_vector(int es, const void* a, int64_t lda, const void* b, int64_t
   return es;
 }
 
-template <typename T, int V>
+template <typename T, int V, int SL, int U>
 static void combine_launch(const void* y, int64_t ldy, const float* w, int T_, int topk, int D, const int* row_of,
                            void* out, int64_t ldo, int sms, cudaStream_t s) {
-  const RowGrid g = row_grid(T_, D / V, sms);
-  combine_kernel<T, V><<<g.grid, g.threads, 0, s>>>(static_cast<const T*>(y), ldy, w, D / V, topk,
-                                                    static_cast<int64_t>(T_) * topk, row_of, static_cast<T*>(out), ldo);
+  const RowGrid g = row_grid(T_, (D / V + U - 1) / U, sms);
+  combine_kernel<T, V, SL, U><<<g.grid, g.threads, 0, s>>>(static_cast<const T*>(y), ldy, w, D / V, topk,
+                                                           static_cast<int64_t>(T_) * topk, row_of, static_cast<T*>(out), ldo);
 }
 
+// Places of the row in flight beside the slots: as many as keep two warps a token
+// busy, and one when few tokens need every thread.
 template <typename T, int V>
+static void combine_wide(const void* y, int64_t ldy, const float* w, int T_, int topk, int D, const int* row_of, void* out,
+                         int64_t ldo, int sms, cudaStream_t s) {
+  const int units = T_ < 2 * sms ? 0 : D / V;
+  if (topk <= 2 && units >= 128)
+    combine_launch<T, V, 2, 2>(y, ldy, w, T_, topk, D, row_of, out, ldo, sms, s);
+  else if (topk <= 4 && units >= 128)
+    combine_launch<T, V, 4, 2>(y, ldy, w, T_, topk, D, row_of, out, ldo, sms, s);
+  else
+    combine_launch<T, V, 8, 1>(y, ldy, w, T_, topk, D, row_of, out, ldo, sms, s);
+}
+
+template <typename T>
+static void combine_rows(bool wide, const void* y, int64_t ldy, const float* w, int T_, int topk, int D, const int* row_of,
+                         void* out, int64_t ldo, int sms, cudaStream_t s) {
+  if (wide)
+    combine_wide<T, 16 / sizeof(T)>(y, ldy, w, T_, topk, D, row_of, out, ldo, sms, s);
+  else
+    combine_launch<T, 1, 8, 1>(y, ldy, w, T_, topk, D, row_of, out, ldo, sms, s);
+}
+
+template <typename T, int V, int SL, int U>
 static void combine_bwd_launch(const void* dout, int64_t ldd, const void* y, int64_t ldy, const float* w, int T_,
                                int topk, int D, const int* row_of, const int* routed, void* dy, int64_t lddy, float* dw,
                                cudaStream_t s) {
-  const int units = D / V, passes = (units + 255) / 256;
+  const int units = (D / V + U - 1) / U, passes = (units + 255) / 256;
   const int threads = ((units + passes - 1) / passes + 31) / 32 * 32;
-  combine_bwd_kernel<T, V><<<static_cast<unsigned>(T_), threads, 0, s>>>(
-      static_cast<const T*>(dout), ldd, static_cast<const T*>(y), ldy, w, units, topk,
+  combine_bwd_kernel<T, V, SL, U><<<static_cast<unsigned>(T_), threads, 0, s>>>(
+      static_cast<const T*>(dout), ldd, static_cast<const T*>(y), ldy, w, D / V, topk,
       static_cast<int64_t>(T_) * topk, row_of, routed, static_cast<T*>(dy), lddy, dw);
+}
+
+template <typename T>
+static void combine_bwd_rows(bool wide, const void* dout, int64_t ldd, const void* y, int64_t ldy, const float* w, int T_,
+                             int topk, int D, const int* row_of, const int* routed, void* dy, int64_t lddy, float* dw,
+                             cudaStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  if (wide && topk <= 2 && D / V >= 128)
+    combine_bwd_launch<T, V, 2, 2>(dout, ldd, y, ldy, w, T_, topk, D, row_of, routed, dy, lddy, dw, s);
+  else if (wide)
+    combine_bwd_launch<T, V, 4, 1>(dout, ldd, y, ldy, w, T_, topk, D, row_of, routed, dy, lddy, dw, s);
+  else
+    combine_bwd_launch<T, 1, 4, 1>(dout, ldd, y, ldy, w, T_, topk, D, row_of, routed, dy, lddy, dw, s);
 }
 
 }  // namespace fack_moe
@@ -715,12 +784,11 @@ int fack_moe_combine(const void* y, int dtype, int64_t ldy, const float* weights
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool wide = row_vector(es, y, ldy, out, ldo, D) == 16;
   if (dtype == FACK_DTYPE_F32)
-    (wide ? combine_launch<float, 4> : combine_launch<float, 1>)(y, ldy, weights, T, topk, D, row_of, out, ldo, sms, s);
+    combine_rows<float>(wide, y, ldy, weights, T, topk, D, row_of, out, ldo, sms, s);
   else if (dtype == FACK_DTYPE_BF16)
-    (wide ? combine_launch<__nv_bfloat16, 8> : combine_launch<__nv_bfloat16, 1>)(y, ldy, weights, T, topk, D, row_of, out,
-                                                                                ldo, sms, s);
+    combine_rows<__nv_bfloat16>(wide, y, ldy, weights, T, topk, D, row_of, out, ldo, sms, s);
   else
-    (wide ? combine_launch<__half, 8> : combine_launch<__half, 1>)(y, ldy, weights, T, topk, D, row_of, out, ldo, sms, s);
+    combine_rows<__half>(wide, y, ldy, weights, T, topk, D, row_of, out, ldo, sms, s);
   return launched();
 }
 
@@ -748,14 +816,11 @@ int fack_moe_combine_bwd(const void* dout, int dtype, int64_t ldd, const void* y
                     (!dy || row_vector(es, dy, lddy, dy, lddy, D) == 16);
   const int* routed = offsets + num_experts;
   if (dtype == FACK_DTYPE_F32)
-    (wide ? combine_bwd_launch<float, 4> : combine_bwd_launch<float, 1>)(dout, ldd, y, ldy, weights, T, topk, D, row_of,
-                                                                        routed, dy, lddy, dweights, s);
+    combine_bwd_rows<float>(wide, dout, ldd, y, ldy, weights, T, topk, D, row_of, routed, dy, lddy, dweights, s);
   else if (dtype == FACK_DTYPE_BF16)
-    (wide ? combine_bwd_launch<__nv_bfloat16, 8> : combine_bwd_launch<__nv_bfloat16, 1>)(
-        dout, ldd, y, ldy, weights, T, topk, D, row_of, routed, dy, lddy, dweights, s);
+    combine_bwd_rows<__nv_bfloat16>(wide, dout, ldd, y, ldy, weights, T, topk, D, row_of, routed, dy, lddy, dweights, s);
   else
-    (wide ? combine_bwd_launch<__half, 8> : combine_bwd_launch<__half, 1>)(dout, ldd, y, ldy, weights, T, topk, D, row_of,
-                                                                          routed, dy, lddy, dweights, s);
+    combine_bwd_rows<__half>(wide, dout, ldd, y, ldy, weights, T, topk, D, row_of, routed, dy, lddy, dweights, s);
   return launched();
 }
 
