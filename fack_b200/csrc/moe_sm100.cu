@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(1024) sort_place_kernel(const I* __restrict__ 
 
 template <int B> struct Bytes;
 template <> struct Bytes<16> { using type = uint4; };
+template <> struct Bytes<8> { using type = uint2; };
 template <> struct Bytes<4> { using type = uint32_t; };
 template <> struct Bytes<2> { using type = uint16_t; };
 
@@ -217,7 +218,7 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// V elements of T moved as one access: 16 bytes as words, or one element.
+// V elements of T moved as one access of 16, 8 or 4 bytes, or one element.
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Pack {
   uint32_t w[V * sizeof(T) / 4];
@@ -226,45 +227,43 @@ template <typename T>
 struct Pack<T, 1> {
   T v;
 };
-template <typename T>
-__device__ __forceinline__ void unpack(const Pack<T, 1>& p, float (&f)[1]) { f[0] = to_f32(p.v); }
-__device__ __forceinline__ void unpack(const Pack<float, 4>& p, float (&f)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(p.w[i]);
+__device__ __forceinline__ void unpack_word(uint32_t w, float* f, __nv_bfloat16*) {
+  f[0] = __uint_as_float(w << 16);
+  f[1] = __uint_as_float(w & 0xffff0000u);
 }
-__device__ __forceinline__ void unpack(const Pack<__nv_bfloat16, 8>& p, float (&f)[8]) {
+__device__ __forceinline__ void unpack_word(uint32_t w, float* f, __half*) {
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  f[0] = v.x;
+  f[1] = v.y;
+}
+__device__ __forceinline__ void unpack_word(uint32_t w, float* f, float*) { f[0] = __uint_as_float(w); }
+__device__ __forceinline__ uint32_t pack_word(const float* f, __nv_bfloat16*) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(f[0], f[1]);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_word(const float* f, __half*) {
+  const __half2 v = __floats2half2_rn(f[0], f[1]);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_word(const float* f, float*) { return __float_as_uint(f[0]); }
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Pack<T, V>& p, float (&f)[V]) {
+  if constexpr (V == 1) {
+    f[0] = to_f32(p.v);
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(p.w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(p.w[i] & 0xffff0000u);
+    for (int i = 0; i < static_cast<int>(V * sizeof(T) / 4); ++i)
+      unpack_word(p.w[i], f + i * (4 / sizeof(T)), static_cast<T*>(nullptr));
   }
 }
-__device__ __forceinline__ void unpack(const Pack<__half, 8>& p, float (&f)[8]) {
+template <typename T, int V>
+__device__ __forceinline__ void pack(Pack<T, V>& p, const float (&f)[V]) {
+  if constexpr (V == 1) {
+    p.v = from_f32<T>(f[0]);
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&p.w[i]));
-    f[2 * i] = v.x;
-    f[2 * i + 1] = v.y;
-  }
-}
-template <typename T>
-__device__ __forceinline__ void pack(Pack<T, 1>& p, const float (&f)[1]) { p.v = from_f32<T>(f[0]); }
-__device__ __forceinline__ void pack(Pack<float, 4>& p, const float (&f)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) p.w[i] = __float_as_uint(f[i]);
-}
-__device__ __forceinline__ void pack(Pack<__nv_bfloat16, 8>& p, const float (&f)[8]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-    p.w[i] = *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-__device__ __forceinline__ void pack(Pack<__half, 8>& p, const float (&f)[8]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-    p.w[i] = *reinterpret_cast<const uint32_t*>(&v);
+    for (int i = 0; i < static_cast<int>(V * sizeof(T) / 4); ++i)
+      p.w[i] = pack_word(f + i * (4 / sizeof(T)), static_cast<T*>(nullptr));
   }
 }
 
@@ -615,7 +614,7 @@ static int sort_launch(const void* ids, int64_t pairs, int E, int* row_of, int* 
 
 // Widest access that every row of both tensors allows.
 static int row_vector(int es, const void* a, int64_t lda, const void* b, int64_t ldb, int D) {
-  for (int v = 16; v > es; v /= 4)
+  for (int v = 16; v > es; v /= 2)
     if (aligned(a, v) && aligned(b, v) && lda * es % v == 0 && ldb * es % v == 0 && static_cast<int64_t>(D) * es % v == 0)
       return v;
   return es;
@@ -644,10 +643,15 @@ static void combine_wide(const void* y, int64_t ldy, const float* w, int T_, int
 }
 
 template <typename T>
-static void combine_rows(bool wide, const void* y, int64_t ldy, const float* w, int T_, int topk, int D, const int* row_of,
+static void combine_rows(int bytes, const void* y, int64_t ldy, const float* w, int T_, int topk, int D, const int* row_of,
                          void* out, int64_t ldo, int sms, cudaStream_t s) {
-  if (wide)
-    combine_wide<T, 16 / sizeof(T)>(y, ldy, w, T_, topk, D, row_of, out, ldo, sms, s);
+  constexpr int es = sizeof(T);
+  if (bytes == 16)
+    combine_wide<T, 16 / es>(y, ldy, w, T_, topk, D, row_of, out, ldo, sms, s);
+  else if (bytes == 8)
+    combine_launch<T, 8 / es, 8, 1>(y, ldy, w, T_, topk, D, row_of, out, ldo, sms, s);
+  else if (bytes == 4)
+    combine_launch<T, 4 / es, 8, 1>(y, ldy, w, T_, topk, D, row_of, out, ldo, sms, s);
   else
     combine_launch<T, 1, 8, 1>(y, ldy, w, T_, topk, D, row_of, out, ldo, sms, s);
 }
@@ -664,14 +668,18 @@ static void combine_bwd_launch(const void* dout, int64_t ldd, const void* y, int
 }
 
 template <typename T>
-static void combine_bwd_rows(bool wide, const void* dout, int64_t ldd, const void* y, int64_t ldy, const float* w, int T_,
+static void combine_bwd_rows(int bytes, const void* dout, int64_t ldd, const void* y, int64_t ldy, const float* w, int T_,
                              int topk, int D, const int* row_of, const int* routed, void* dy, int64_t lddy, float* dw,
                              cudaStream_t s) {
-  constexpr int V = 16 / sizeof(T);
-  if (wide && topk <= 2 && D / V >= 128)
+  constexpr int es = sizeof(T), V = 16 / es;
+  if (bytes == 16 && topk <= 2 && D / V >= 128)
     combine_bwd_launch<T, V, 2, 2>(dout, ldd, y, ldy, w, T_, topk, D, row_of, routed, dy, lddy, dw, s);
-  else if (wide)
+  else if (bytes == 16)
     combine_bwd_launch<T, V, 4, 1>(dout, ldd, y, ldy, w, T_, topk, D, row_of, routed, dy, lddy, dw, s);
+  else if (bytes == 8)
+    combine_bwd_launch<T, 8 / es, 4, 1>(dout, ldd, y, ldy, w, T_, topk, D, row_of, routed, dy, lddy, dw, s);
+  else if (bytes == 4)
+    combine_bwd_launch<T, 4 / es, 4, 1>(dout, ldd, y, ldy, w, T_, topk, D, row_of, routed, dy, lddy, dw, s);
   else
     combine_bwd_launch<T, 1, 4, 1>(dout, ldd, y, ldy, w, T_, topk, D, row_of, routed, dy, lddy, dw, s);
 }
@@ -734,6 +742,8 @@ int fack_moe_gather(const void* x, int dtype, int64_t ldx, int T, int topk, int 
   const int* routed = offsets + num_experts;
   if (b == 16)
     gather_kernel<16><<<g.grid, g.threads, 0, s>>>(x, ldx * es / 16, units, topk, rows, row_of, routed, y, ldy * es / 16);
+  else if (b == 8)
+    gather_kernel<8><<<g.grid, g.threads, 0, s>>>(x, ldx * es / 8, units, topk, rows, row_of, routed, y, ldy * es / 8);
   else if (b == 4)
     gather_kernel<4><<<g.grid, g.threads, 0, s>>>(x, ldx * es / 4, units, topk, rows, row_of, routed, y, ldy * es / 4);
   else
@@ -782,13 +792,13 @@ int fack_moe_combine(const void* y, int dtype, int64_t ldy, const float* weights
   st = fack::sm100_device(&sms);
   if (st != FACK_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool wide = row_vector(es, y, ldy, out, ldo, D) == 16;
+  const int bytes = row_vector(es, y, ldy, out, ldo, D);
   if (dtype == FACK_DTYPE_F32)
-    combine_rows<float>(wide, y, ldy, weights, T, topk, D, row_of, out, ldo, sms, s);
+    combine_rows<float>(bytes, y, ldy, weights, T, topk, D, row_of, out, ldo, sms, s);
   else if (dtype == FACK_DTYPE_BF16)
-    combine_rows<__nv_bfloat16>(wide, y, ldy, weights, T, topk, D, row_of, out, ldo, sms, s);
+    combine_rows<__nv_bfloat16>(bytes, y, ldy, weights, T, topk, D, row_of, out, ldo, sms, s);
   else
-    combine_rows<__half>(wide, y, ldy, weights, T, topk, D, row_of, out, ldo, sms, s);
+    combine_rows<__half>(bytes, y, ldy, weights, T, topk, D, row_of, out, ldo, sms, s);
   return launched();
 }
 
@@ -811,16 +821,22 @@ int fack_moe_combine_bwd(const void* dout, int dtype, int64_t ldd, const void* y
   st = fack::sm100_device(&sms);
   if (st != FACK_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool wide = row_vector(es, dout, ldd, dout, ldd, D) == 16 &&
-                    (!dweights || row_vector(es, y, ldy, y, ldy, D) == 16) &&
-                    (!dy || row_vector(es, dy, lddy, dy, lddy, D) == 16);
+  int bytes = row_vector(es, dout, ldd, dout, ldd, D);
+  if (dweights) {
+    const int b = row_vector(es, y, ldy, y, ldy, D);
+    bytes = b < bytes ? b : bytes;
+  }
+  if (dy) {
+    const int b = row_vector(es, dy, lddy, dy, lddy, D);
+    bytes = b < bytes ? b : bytes;
+  }
   const int* routed = offsets + num_experts;
   if (dtype == FACK_DTYPE_F32)
-    combine_bwd_rows<float>(wide, dout, ldd, y, ldy, weights, T, topk, D, row_of, routed, dy, lddy, dweights, s);
+    combine_bwd_rows<float>(bytes, dout, ldd, y, ldy, weights, T, topk, D, row_of, routed, dy, lddy, dweights, s);
   else if (dtype == FACK_DTYPE_BF16)
-    combine_bwd_rows<__nv_bfloat16>(wide, dout, ldd, y, ldy, weights, T, topk, D, row_of, routed, dy, lddy, dweights, s);
+    combine_bwd_rows<__nv_bfloat16>(bytes, dout, ldd, y, ldy, weights, T, topk, D, row_of, routed, dy, lddy, dweights, s);
   else
-    combine_bwd_rows<__half>(wide, dout, ldd, y, ldy, weights, T, topk, D, row_of, routed, dy, lddy, dweights, s);
+    combine_bwd_rows<__half>(bytes, dout, ldd, y, ldy, weights, T, topk, D, row_of, routed, dy, lddy, dweights, s);
   return launched();
 }
 

@@ -195,7 +195,7 @@ def test_gradients_that_autograd_hands_out_broadcast_or_transposed(cuda_device):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("off,width", [(0, 80), (1, 77), (2, 72), (8, 88)])
+@pytest.mark.parametrize("off,width", [(0, 80), (1, 77), (2, 72), (8, 88), (4, 76), (0, 66), (0, 68)])
 def test_strided_and_unaligned_rows(cuda_device, dtype, off, width):
     T, k, E, D = 20, 3, 5, 64
     plan = gpu_plan(T, k, E, off, cuda_device)
