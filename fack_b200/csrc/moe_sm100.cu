@@ -276,7 +276,8 @@ __device__ __forceinline__ void zero_tail(U* y, int64_t ldy, int nvec, int64_t r
     for (int v = blockIdx.y * blockDim.x + threadIdx.x; v < nvec; v += gridDim.y * blockDim.x) y[r * ldy + v] = zero;
 }
 
-// y[row_of[t, j]] = x[t], as bytes.  One block (or gridDim.y blocks) a token.
+// y[row_of[t, j]] = x[t], as bytes.  One block (or gridDim.y blocks) a token; the
+// next bytes of x are on their way while the last are written.
 template <int B>
 __global__ void __launch_bounds__(256) gather_kernel(const void* __restrict__ xp, int64_t ldx, int nvec, int topk,
                                                      int64_t rows, const int* __restrict__ row_of,
@@ -287,13 +288,17 @@ __global__ void __launch_bounds__(256) gather_kernel(const void* __restrict__ xp
   const U* x = static_cast<const U*>(xp);
   U* y = static_cast<U*>(yp);
   const int64_t t = blockIdx.x;
+  const int step = gridDim.y * blockDim.x;
+  int v = blockIdx.y * blockDim.x + threadIdx.x;
+  U next = v < nvec ? x[t * ldx + v] : U{};       // on its way while the rows are looked up
   for (int j = threadIdx.x; j < topk; j += blockDim.x) {
     const int r = row_of[t * topk + j];
     at[j] = r >= 0 && r < rows ? r : -1;
   }
   __syncthreads();
-  for (int v = blockIdx.y * blockDim.x + threadIdx.x; v < nvec; v += gridDim.y * blockDim.x) {
-    const U val = x[t * ldx + v];
+  for (; v < nvec; v += step) {
+    const U val = next;
+    if (v + step < nvec) next = x[t * ldx + v + step];
 #pragma unroll 4
     for (int j = 0; j < topk; ++j) {
       const int r = at[j];
