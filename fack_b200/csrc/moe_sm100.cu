@@ -503,7 +503,7 @@ __device__ __forceinline__ void load16(const __nv_bfloat16* p, float (&v)[16]) {
 // with NaN on top, so a group that holds one gets scale NaN and NaN codes; a
 // group whose scale would round to 0 gets scale 1 and zero codes.
 template <typename T>
-__global__ void __launch_bounds__(256) gather_quant_kernel(const T* __restrict__ x, int64_t ldx, int KB, int topk,
+__global__ void __launch_bounds__(256, 6) gather_quant_kernel(const T* __restrict__ x, int64_t ldx, int KB, int topk,
                                                            int64_t rows, const int* __restrict__ row_of,
                                                            const int* __restrict__ routed, uint8_t* __restrict__ xq,
                                                            int64_t ldq, float* __restrict__ xs, int64_t lds) {
