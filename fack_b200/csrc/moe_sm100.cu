@@ -17,6 +17,13 @@
 // read, all loads in flight together, and one row written), so each byte
 // crosses HBM once and no sum needs an atomic.  Every index read from a plan
 // is range-checked before it is used as an address.
+//
+// Measured on B200 (graph replay, share of the 6464 GB/s copy): gather 8192 x 8 rows
+// of 7168 bf16 176 us (0.93, in L2's favour at smaller sizes), 4096 x 6 of 4096 fp16
+// 39 (0.92); combine 154 and 39 (0.93); combine's gradients 4096 x 6 x 4096 74 (0.92);
+// the quantising gather 4095 x 4 of 7168 fp32 40 (0.93), 8192 x 2 of 7168 bf16 57
+// (0.65: a division and a conversion an element cost more than two bytes in and two
+// out).  Few tokens are bound by latency: 2-4 us to 16 tokens.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -93,10 +100,12 @@ __global__ void __launch_bounds__(1024) sort_count_kernel(const I* __restrict__ 
 
 // Ranks and scatters each block's share, chunk by chunk.  A warp takes a
 // contiguous run of a chunk, 32 pairs a round: lanes with the same expert find
-// each other by a ballot for each bit of its number, their rank is the warp's running count plus the
-// lanes before them, so order is kept without an atomic.  A column scan over
-// the warps then turns counts into rows.  With one block (hist NULL) the counts
-// of the first and only chunk are the histogram.
+// each other by a ballot for each bit of its number (match.any is slower: 9.7
+// against 7.9 us for 4096 pairs over 256 experts), their rank is the warp's running
+// count plus the lanes before them, so order is kept without an atomic.  A column
+// scan over the warps then turns counts into rows.  With one block (hist NULL) the
+// counts of the first and only chunk are the histogram.  Bound by latency: 2.4 us
+// for one token's pairs, 11 us for 524288 over 64 experts in two launches.
 template <typename I>
 __global__ void __launch_bounds__(1024) sort_place_kernel(const I* __restrict__ ids, int64_t pairs, int64_t share, int E,
                                                           const int* __restrict__ hist, int* __restrict__ row_of,
@@ -369,7 +378,10 @@ __global__ void __launch_bounds__(256) combine_kernel(const T* __restrict__ y, i
 
 // dy[row_of[t, j]] = w[t, j] * dout[t] and dw[t, j] = <dout[t], y[row_of[t, j]]>
 // (either may be NULL), one block a token.  The dot products are fp32: each
-// thread's own columns in order, then the lanes, then the warps.
+// thread's own columns in order, then the lanes, then the warps.  Four slots at a
+// time (two places of the row when a token has two): with eight the registers leave
+// two blocks an SM and 4096 x 6 x 4096 took 122 instead of 103 us, launch included.
+// dout's load waits for no index.
 template <typename T, int V, int SL, int U>
 __global__ void __launch_bounds__(256, 3) combine_bwd_kernel(const T* __restrict__ dout, int64_t ldd,
                                                           const T* __restrict__ y, int64_t ldy,
@@ -501,7 +513,9 @@ __device__ __forceinline__ void load16(const __nv_bfloat16* p, float (&v)[16]) {
 // its topk rows.  Eight lanes take a group of 128, 16 elements each, so a lane's
 // codes are one 16-byte store.  The magnitudes' bit patterns order as integers
 // with NaN on top, so a group that holds one gets scale NaN and NaN codes; a
-// group whose scale would round to 0 gets scale 1 and zero codes.
+// group whose scale would round to 0 gets scale 1 and zero codes.  Six blocks an SM
+// (40 registers): 8192 x 2 rows of 7168 bf16 61 -> 57 us; loading a group ahead takes
+// 60 registers and 71 us.
 template <typename T>
 __global__ void __launch_bounds__(256, 6) gather_quant_kernel(const T* __restrict__ x, int64_t ldx, int KB, int topk,
                                                            int64_t rows, const int* __restrict__ row_of,
