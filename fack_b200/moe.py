@@ -219,7 +219,7 @@ def _refuse_captured_leaf(*inputs) -> None:
     """No gradient of a leaf inside a CUDA-graph capture: where an eager graph of
     the same leaf is alive, autograd would make the capture wait on that graph's
     stream, which ends the process.  The backward functions have no such state."""
-    if torch.cuda.is_current_stream_capturing() and any(t.requires_grad and t.is_leaf for t in inputs):
+    if any(t.is_cuda and t.requires_grad and t.is_leaf for t in inputs) and torch.cuda.is_current_stream_capturing():
         raise ValueError("a captured gather or combine takes no leaf that requires grad; call moe_gather_backward / "
                          "moe_combine_backward in the capture instead, or detach the input")
 
