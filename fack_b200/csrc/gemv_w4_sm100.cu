@@ -509,7 +509,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
                 mma_step<T>(d[r][n], false, l[2], h[2], l[3], h[3], b[n][2], b[n][3]);
               }
             }
-            if ((j + 1) * 32 % FL == 0) {
+            // (a group past K is the next expert's: its scale may be infinite)
+            if ((j + 1) * 32 % FL == 0 && (FL == 128 || j * 32 < left)) {
               const uint32_t sp = st + s_at + (srow + j * 32 / FL) * box_rows * es;
               float scale[R][2];
               if (p.scale_f32) {

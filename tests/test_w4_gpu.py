@@ -364,3 +364,17 @@ def test_a_stack_of_most_experts(cuda_device):
     row_of, src, offsets = moe_orc.sort_ref(ids, E)
     ref = orc.experts_ref(moe_orc.gather_ref(x, src, 2), w, s, None, offsets, 10)[0]
     assert torch.equal(fb.gemv_w4_experts(*to(cuda_device, x, w, s), plan).cpu().double(), ref)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K,G", [(160, 32), (32, 32), (64, 64), (192, 64)])
+def test_the_next_experts_scales_are_not_met(cuda_device, dtype, K, G):
+    """K ends inside a block of 128: what lies behind it belongs to the next expert."""
+    E, N = 3, 48
+    w, s, z = weight((E,), N, K, G, True, torch.float32, K, exact=True)
+    x, ids = few_ones(4, K, K, dtype), torch.tensor([[0], [2], [0], [2]])
+    s[1] = float("inf")
+    plan = moe_orc.sort_ref(ids, E)
+    ref, _ = orc.experts_ref(x[plan[1].long()], w, s, z, plan[2], 4)
+    y = fb.gemv_w4_experts(*to(cuda_device, x, w, s), fb.MoePlan(*to(cuda_device, *plan)), to(cuda_device, z)[0])
+    assert torch.equal(y.cpu().double(), ref)
