@@ -25,12 +25,15 @@
 //     into the next.  Rows per warp, slices and rows per item follow a cost model
 //     (see plan): few rows are split along K, many are dealt out evenly.
 // Measured on B200, L2 flushed: 65536 x 7168 (235 MB) with one token 55 us = 4.3 TB/s,
-// with eight 58 us, with thirteen 90-98 us; the copies alone take 43-46 us (55-61 with
-// thirteen).  ncu there: 15 instructions a word, 53 % of the issue slots, ALU 45 %,
-// tensor pipe 27 %, DRAM 60 %: bound by the unpacking's latency and issue.
-// The warp MMA, not tcgen05: 8 or 16 tokens fill a fraction of a tcgen05 tile,
-// 4-bit codes with arbitrary scales are no operand type of it, and dequantised
-// tiles would have to pass through shared memory once more.  Tokens in three 8-bit
+// with eight 58 us, with thirteen 85-91 us; the copies alone take 43-46 us (55-61 with
+// thirteen).  ncu with one: 20 instructions a word in all, 60 % of the issue slots; with
+// thirteen 25 and 53 %, most stalls on results of the instructions before: bound by
+// the latency and issue of the unpacking.
+// The warp MMA, not tcgen05: a form that unpacks into tensor memory (the codes as A,
+// 128 rows x 64 k a step, sixteen warps) was built and gave 88-94 us for one token and
+// 94-106 for thirteen.  Its products cost next to nothing (9 cycles for 128 x 16 x 16),
+// but a lane then unpacks as much, adds 16 sums a group instead of 8, and pays stores,
+// loads and waits of tensor memory: 32 instructions a word.  Tokens in three 8-bit
 // digits and codes as they are (exact, a third of the unpacking) were measured with
 // the int8 MMA (56 / 71 / 126 us for 1 / 8 / 13 tokens: three times the MMAs and
 // accumulators) and the fp8 MMA (92 us: mma.sync converts its operands here).
@@ -42,6 +45,7 @@
 #include <stdint.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "../../include/fack_gemm.h"
 #include "fack_internal.h"
@@ -449,101 +453,111 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.0f;
-      for (int kb0 = 0; kb0 < KB; kb0 += split) {
-        if (alive) alive = wait_bounded(smem_addr(&full[s]), phase, abort_flag, p.status, kStW4, p.timeout_ns);
-        __syncwarp();
-        const int kb = kb0 + slice;
-        if (kb < KB) {
-          const uint32_t st = ring + s * stage_bytes;
-          const int left = p.K - kb * kBlkK;    // k of this block inside K
-          // the block's first row of scales: its own, or that of the group it lies in
-          int srow = slice * S::kGroups;
-          if (FL == 128 && p.G != 128)
-            srow = kb * kBlkK / p.G - kb0 * kBlkK / p.G;
-          float d[R][NT][4];
-          uint32_t mz[R][2];                    // minus the zero points of rows g, g + 8
-          uint32_t wl[R][S::kWords], wh[R][S::kWords];   // their words
-#pragma unroll (R == 4 && NT == 1 && (FL == 32 || (FL == 64 && ZP)) ? FL / 32 : 4)
-          for (int j = 0; j < 4; ++j) {         // 32 k each
-            const bool first = j * 32 % FL == 0;
-            if (first) {
-              const uint32_t zp = st + z_at + (srow + j * 32 / FL) * box_rows;
+      // the item's K, this warp's R or R - 1 groups of rows.  With groups of 32 or 64 k the
+      // loop is compiled for either (a test for the last rows inside it: 65536 x 7168, 13
+      // tokens, G = 64, 98 us, now 90); with 128 two loops need more registers (R = 4: 55 -> 57).
+      auto multiply = [&](auto groups_here) {
+        constexpr int RR = decltype(groups_here)::value;
+        for (int kb0 = 0; kb0 < KB; kb0 += split) {
+          if (alive) alive = wait_bounded(smem_addr(&full[s]), phase, abort_flag, p.status, kStW4, p.timeout_ns);
+          __syncwarp();
+          const int kb = kb0 + slice;
+          if (kb < KB) {
+            const uint32_t st = ring + s * stage_bytes;
+            const int left = p.K - kb * kBlkK;    // k of this block inside K
+            // the block's first row of scales: its own, or that of the group it lies in
+            int srow = slice * S::kGroups;
+            if (FL == 128 && p.G != 128)
+              srow = kb * kBlkK / p.G - kb0 * kBlkK / p.G;
+            float d[RR][NT][4];
+            uint32_t mz[RR][2];                    // minus the zero points of rows g, g + 8
+            uint32_t wl[RR][S::kWords], wh[RR][S::kWords];   // their words
+#pragma unroll (RR == 4 && NT == 1 && (FL == 32 || (FL == 64 && ZP)) ? FL / 32 : 4)
+            for (int j = 0; j < 4; ++j) {         // 32 k each
+              // past K: no tokens there, and the next expert's scales, which may be infinite
+              if (FL < 128 && j / S::kWords * S::kWords * 32 >= left) break;
+              const bool first = j * 32 % FL == 0;
+              if (first) {
+                const uint32_t zp = st + z_at + (srow + j * 32 / FL) * box_rows;
 #pragma unroll
-              for (int r = 0; r < R; ++r) {
-                mz[r][0] = mz[r][1] = C::kMinusEight;
-                if (ZP) {
-                  mz[r][0] = mul2<T>((lds8(zp + r * 16) & 15u) * 0x00010001u, C::kNegate);
-                  mz[r][1] = mul2<T>((lds8(zp + r * 16 + 8) & 15u) * 0x00010001u, C::kNegate);
+                for (int r = 0; r < RR; ++r) {
+                  mz[r][0] = mz[r][1] = C::kMinusEight;
+                  if (ZP) {
+                    mz[r][0] = mul2<T>((lds8(zp + r * 16) & 15u) * 0x00010001u, C::kNegate);
+                    mz[r][1] = mul2<T>((lds8(zp + r * 16 + 8) & 15u) * 0x00010001u, C::kNegate);
+                  }
                 }
               }
-            }
-            const int chunk = 4 * S::kWords * (j / S::kWords) + j % S::kWords;   // + WV q: the lane's 8 k
-            uint32_t b[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              uint4 v = lds128(st + x_at[n] + chunk * 16);
-              if (FL < 128 && (chunk + S::kWords * q) * 8 >= left) v = make_uint4(0, 0, 0, 0);   // past K: not brought
-              b[n][0] = __byte_perm(v.x, v.z, 0x5410);      // x0, x4
-              b[n][1] = __byte_perm(v.x, v.z, 0x7632);      // x1, x5
-              b[n][2] = __byte_perm(v.y, v.w, 0x5410);      // x2, x6
-              b[n][3] = __byte_perm(v.y, v.w, 0x7632);      // x3, x7
-            }
-            if (j % S::kWords == 0) {
-              // part j / WV: 16 bytes on (WV = 1), 32 bytes on (WV = 2)
-              const uint32_t wj = (st + w_at) ^ (S::kWords == 1 ? j << 4 : (j >> 1) << 5);
-#pragma unroll
-              for (int r = 0; r < R; ++r) {
-                lds_words(wj + r * 1024, wl[r]);
-                lds_words(wj + r * 1024 + 512, wh[r]);
-              }
-            }
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-              if (r == R - 1 && !full_part) break;
-              uint32_t l[4], h[4];
-              unpack_codes<T>(wl[r][j % S::kWords], mz[r][0], l);
-              unpack_codes<T>(wh[r][j % S::kWords], mz[r][1], h);
+              const int chunk = 4 * S::kWords * (j / S::kWords) + j % S::kWords;   // + WV q: the lane's 8 k
+              uint32_t b[NT][4];
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                mma_step<T>(d[r][n], first, l[0], h[0], l[1], h[1], b[n][0], b[n][1]);
-                mma_step<T>(d[r][n], false, l[2], h[2], l[3], h[3], b[n][2], b[n][3]);
+                const uint4 v = lds128(st + x_at[n] + chunk * 16);
+                b[n][0] = __byte_perm(v.x, v.z, 0x5410);      // x0, x4
+                b[n][1] = __byte_perm(v.x, v.z, 0x7632);      // x1, x5
+                b[n][2] = __byte_perm(v.y, v.w, 0x5410);      // x2, x6
+                b[n][3] = __byte_perm(v.y, v.w, 0x7632);      // x3, x7
               }
-            }
-            // (a group past K is the next expert's: its scale may be infinite)
-            if ((j + 1) * 32 % FL == 0 && (FL == 128 || j * 32 < left)) {
-              const uint32_t sp = st + s_at + (srow + j * 32 / FL) * box_rows * es;
-              float scale[R][2];
-              if (p.scale_f32) {
+              if (j % S::kWords == 0) {
+                // part j / WV: 16 bytes on (WV = 1), 32 bytes on (WV = 2)
+                const uint32_t wj = (st + w_at) ^ (S::kWords == 1 ? j << 4 : (j >> 1) << 5);
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                  scale[r][0] = __uint_as_float(lds32(sp + r * 64));
-                  scale[r][1] = __uint_as_float(lds32(sp + r * 64 + 32));
-                }
-              } else {
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                  scale[r][0] = scale_of(lds16(sp + r * 32), static_cast<T*>(nullptr));
-                  scale[r][1] = scale_of(lds16(sp + r * 32 + 16), static_cast<T*>(nullptr));
+                for (int r = 0; r < RR; ++r) {
+                  lds_words(wj + r * 1024, wl[r]);
+                  lds_words(wj + r * 1024 + 512, wh[r]);
                 }
               }
 #pragma unroll
-              for (int r = 0; r < R; ++r) {
-                if (r == R - 1 && !full_part) break;
+              for (int r = 0; r < RR; ++r) {
+                if (FL == 128 && r == R - 1 && !full_part) break;
+                uint32_t l[4], h[4];
+                unpack_codes<T>(wl[r][j % S::kWords], mz[r][0], l);
+                unpack_codes<T>(wh[r][j % S::kWords], mz[r][1], h);
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n) {
+                  mma_step<T>(d[r][n], first, l[0], h[0], l[1], h[1], b[n][0], b[n][1]);
+                  mma_step<T>(d[r][n], false, l[2], h[2], l[3], h[3], b[n][2], b[n][3]);
+                }
+              }
+              if ((j + 1) * 32 % FL == 0) {
+                const uint32_t sp = st + s_at + (srow + j * 32 / FL) * box_rows * es;
+                float scale[RR][2];
+                if (p.scale_f32) {
 #pragma unroll
-                  for (int i = 0; i < 4; ++i) acc[r][n][i] = fmaf(scale[r][i / 2], d[r][n][i], acc[r][n][i]);
+                  for (int r = 0; r < RR; ++r) {
+                    scale[r][0] = __uint_as_float(lds32(sp + r * 64));
+                    scale[r][1] = __uint_as_float(lds32(sp + r * 64 + 32));
+                  }
+                } else {
+#pragma unroll
+                  for (int r = 0; r < RR; ++r) {
+                    scale[r][0] = scale_of(lds16(sp + r * 32), static_cast<T*>(nullptr));
+                    scale[r][1] = scale_of(lds16(sp + r * 32 + 16), static_cast<T*>(nullptr));
+                  }
+                }
+#pragma unroll
+                for (int r = 0; r < RR; ++r) {
+                  if (FL == 128 && r == R - 1 && !full_part) break;
+#pragma unroll
+                  for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[r][n][i] = fmaf(scale[r][i / 2], d[r][n][i], acc[r][n][i]);
+                }
               }
             }
           }
+          __syncwarp();                           // every lane has read the stage
+          if (lane == 0) mbar_arrive(smem_addr(&empty[s]));
+          if (++s == p.stages) {
+            s = 0;
+            phase ^= 1u;
+          }
         }
-        __syncwarp();                           // every lane has read the stage
-        if (lane == 0) mbar_arrive(smem_addr(&empty[s]));
-        if (++s == p.stages) {
-          s = 0;
-          phase ^= 1u;
-        }
-      }
+      };
+      if (FL == 128 || full_part)
+        multiply(std::integral_constant<int, R>());
+      else
+        multiply(std::integral_constant<int, R - 1>());
       const unsigned rows_with_x = __ballot_sync(0xffffffffu, lane < it.count && x_row_of(it.row0 + lane) >= 0);
       T* y = static_cast<T*>(p.y) + static_cast<int64_t>(it.row0) * p.ldy;
       if (split == 1) {
@@ -607,10 +621,13 @@ struct Plan {
 };
 
 // Rounds of `items` over `at_once` places.  Where the number of items is a guess
-// (`about`), a last round is on average half empty whatever the sizes.
+// (`about`), the mean over guesses up to 9 % off.
 static double rounds(double items, int at_once, bool about) {
   const double r = items / at_once;
-  return !about ? ceil(r) : r < 0.8 ? 1.0 : r + 0.6;
+  if (!about) return ceil(r);
+  double sum = 0.0;
+  for (int off = -9; off <= 9; off += 3) sum += ceil(r * (1.0 + 0.01 * off));
+  return sum / 7.0;
 }
 
 // The cheapest R, split and item for `tiles` token tiles of up to 8 NT tokens.
@@ -622,9 +639,9 @@ static double rounds(double items, int at_once, bool about) {
 // 68; 7168 x 2048: R = 2 with eight slices 10-11, R = 4 12; 8192 x 7168, 16 tokens:
 // R = 4 22, R = 2 29.)
 // Items need not be full: N = 65536 makes 256 items of 256 rows, two on 108 SMs and
-// one on 40, but 293 of 224 rows, two on nearly all (58 -> 55 us).  With groups below
-// 128 the branch around a warp's last rows costs more than that (137 -> 172 us for 64
-// experts of 7168 x 2048), so there they stay full.
+// one on 40, but 293 of 224 rows, two on nearly all (58 -> 55 us with one token).  A
+// warp's last rows cost about half as much as the mean (its other rows hide them).
+// Over 59 calls the plan was 1.7 % slower than the best of all plans (mean; 20 % at most).
 static Plan plan(int NT, double tiles, bool about, int N, int K, int G, int sms) {
   Plan best = {2, kWarps, 2, 1e30};
   const int KB = (K + kBlkK - 1) / kBlkK;
@@ -634,11 +651,11 @@ static Plan plan(int NT, double tiles, bool about, int N, int K, int G, int sms)
     for (int split = kWarps; split >= 1; split /= 2) {
       const int share = kWarps / split, steps = (KB + split - 1) / split;
       const double join = split == kWarps ? (R == 2 ? 1.0 : 1.7) : split > 1 ? 0.8 : 0.3;
-      const int least = G % 128 ? R * share : (R - 1) * share + 1;
+      const int least = (R - 1) * share + 1;
       for (int groups = R * share; groups >= least; --groups) {
         if (groups > 16 && (groups % 2 || groups / 2 <= (R - 1) * (share / 2))) continue;   // two even boxes
         const double items = tiles * ((N / 16 + groups - 1) / groups);
-        const double work = steps * step * groups / (R * share);
+        const double work = steps * step * (0.5 + 0.5 * groups / (R * share));
         const double busy = rounds(items, sms, about) * (work + join);
         const double alone = rounds(items, sms * ctas, about) * (0.8 * ctas * work + join);
         const double us = busy > alone ? busy : alone;
@@ -726,7 +743,7 @@ static double expected_tiles(int T, int topk, int E, int tile) {
 }
 
 // Tokens per tile (8 NT at most) and the plan.  An expert's rows are known on the
-// device alone; it is not likely to have more than there are tokens.
+// device alone; it is not likely to have more than there are tokens, and one token has topk.
 static void choose(Args& a, int tokens, int sms, int* NT, int* R) {
   Plan p[2];
   int tile[2];
@@ -741,7 +758,7 @@ static void choose(Args& a, int tokens, int sms, int* NT, int* R) {
       tile[i] = static_cast<int>((a.rows + n - 1) / n);      // evenly filled
       tiles = static_cast<double>(n);
     }
-    p[i] = plan(i + 1, tiles, a.offsets != nullptr, a.N, a.K, a.G, sms);
+    p[i] = plan(i + 1, tiles, a.offsets != nullptr && tokens > 1, a.N, a.K, a.G, sms);
   }
   const int i = tile[1] > 8 && p[1].us < p[0].us;
   *NT = i + 1;
