@@ -56,6 +56,8 @@ def _check_out(out, rows: int, N: int, x):
     if not isinstance(out, torch.Tensor) or out.dtype != x.dtype or tuple(out.shape) != (rows, N) or out.stride(1) != 1 \
             or out.device != x.device or (rows > 1 and out.stride(0) < N):
         raise ValueError(f"out must be a {x.dtype} [{rows}, {N}] tensor with unit column stride on {x.device}")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("out is written outside autograd: it must not require grad")
     return out
 
 
@@ -64,7 +66,7 @@ def gemv_w4(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, zeros: Optio
     """y [M, N] = x [M, K] (bf16 or fp16, rows 16-byte aligned) times the 4-bit
     weight ``w`` [N, K/2] transposed.  Any M is right; the kernel is made for
     the M up to about 32 of a decode step (more tokens are taken 8 or 16 at a
-    time).  Writes and returns ``out`` when given."""
+    time).  Writes and returns ``out`` when given (it may not overlap an operand)."""
     _check_rows(x, "x", dtypes=TYPES)
     N, K, G = _check_weight(x, w, scales, zeros, ())
     M = x.shape[0]
@@ -83,7 +85,8 @@ def gemv_w4_experts(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, plan
     [E, K/G, N].  ``x`` is the tokens [T, K], gathered on the way in, or with
     ``sorted_rows`` the rows [T*k, K] in sorted order (an earlier product's
     output).  Rows without a pair are written as zeros.  Only the experts that
-    have rows are read; the row counts stay on the device."""
+    have rows are read; the row counts stay on the device.  Writes and returns
+    ``out`` when given (it may not overlap an operand)."""
     _check_rows(x, "x", dtypes=TYPES)
     T, topk, E = _check_plan(plan, x.device)
     N, K, G = _check_weight(x, w, scales, zeros, (E,))

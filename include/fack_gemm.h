@@ -469,7 +469,8 @@ int fack_gemm_tn(int kind, const void* a, int64_t lda, const void* b, int b_pack
  * row) and run on FACK_DTYPE_F32, _BF16 or _F16 rows of D elements,
  * 1 <= D <= 2^20, in any alignment of the element type; rows that allow 16-byte
  * accesses (base, stride and D) go faster.  Sorted buffers hold T*topk rows; rows
- * without a pair are written as zeros (their scales as 1).
+ * without a pair are written as zeros (their scales as 1).  No output may overlap
+ * an input or have rows that overlap.
  *
  *   fack_moe_gather        y[row_of[t, j]] = x[t]
  *   fack_moe_gather_quant  xq, x_scale of row row_of[t, j] = the e4m3 codes and
@@ -515,7 +516,7 @@ int fack_moe_combine_bwd(const void* dout, int dtype, int64_t ldd, const void* y
  * G = 32, 64 or a multiple of 128; K % G == 0, K <= 2^20; M >= 1 (meant for M
  * up to about 32: more tokens are taken 8 or 16 at a time).  Products are exact, sums
  * fp32, one rounding to y's type; the same call gives the same bits.
- * Capturable; allocates nothing.
+ * Capturable; allocates nothing.  y may not overlap an operand.
  *
  * fack_gemv_w4_experts: y [T*topk, N] from the weights of each sorted row's
  * expert: w [E, N, K/2], scales and zeros [E, K/G, N], offsets (and src) of a

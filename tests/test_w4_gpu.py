@@ -378,3 +378,15 @@ def test_the_next_experts_scales_are_not_met(cuda_device, dtype, K, G):
     ref, _ = orc.experts_ref(x[plan[1].long()], w, s, z, plan[2], 4)
     y = fb.gemv_w4_experts(*to(cuda_device, x, w, s), fb.MoePlan(*to(cuda_device, *plan)), to(cuda_device, z)[0])
     assert torch.equal(y.cpu().double(), ref)
+
+
+def test_an_out_that_requires_grad_is_refused(cuda_device):
+    w, s, _ = to(cuda_device, *weight((), 32, 64, 64, False, torch.float32, 1))
+    x = torch.ones((2, 64), device=cuda_device).bfloat16()
+    out = torch.zeros((2, 32), device=cuda_device, dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(ValueError, match="out"):
+        fb.gemv_w4(x, w, s, out=out)
+    assert (out == 0).all()
+    with torch.no_grad():
+        assert fb.gemv_w4(x, w, s, out=out) is out
+    assert torch.equal(out.detach(), fb.gemv_w4(x, w, s))
