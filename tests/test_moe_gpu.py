@@ -429,3 +429,18 @@ def test_sort_quantise_gemm_combine(cuda_device):
     ref, mag = orc.combine_ref(ry, w, row_of)
     # the GEMM's own tolerance (rtol = atol = 1e-2 before the combine), weights below 1, two rows a token
     close(out, ref, 1e-2 * mag + 1e-2 * k + rounding(torch.bfloat16, ref))
+
+
+def test_gradients_of_gradients_are_refused(cuda_device):
+    """create_graph gives the first gradients as usual; a second derivative through
+    them is an error, not a silent zero."""
+    ids = torch.tensor([[0, 1], [1, 2]], device=cuda_device)
+    plan = fb.moe_sort(ids, 3)
+    x = torch.randn((2, 8), device=cuda_device, requires_grad=True)
+    y = torch.randn((4, 8), device=cuda_device, requires_grad=True)
+    gates = torch.rand((2, 2), device=cuda_device, requires_grad=True)
+    for out, leaf in ((fb.moe_gather(x, plan), x), (fb.moe_combine(y, gates, plan), gates)):
+        g = torch.randn_like(out, requires_grad=True)
+        first, = torch.autograd.grad(out, leaf, g, create_graph=True)
+        with pytest.raises(RuntimeError):
+            first.sum().backward()
