@@ -435,6 +435,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
     const int in_box = box ? parts - 1 - part_no % parts : part_no % parts;
     const int box_row = 16 * (in_box * each + min(in_box, more)), first_row = box * box_rows + box_row;
     const bool full_part = each + (in_box < more ? 1 : 0) == R;
+    // With groups of 128 k a part of R - 1 groups loads for a last one as well, whose products are
+    // left out.  Its words lie in the stage; behind the last box of scales or zero points the
+    // ring may end, so there it loads those of the group before.
+    const uint32_t last = full_part ? R - 1 : R - 2;
+    auto loaded = [&](int r) -> uint32_t { return FL == 128 && r == R - 1 ? last : r; };
     const uint32_t w_at = slice * item_rows * 64 + (first_row + g) * 64 +
                           (((S::kWords == 1 ? 0 : q >> 1) ^ ((g >> 1) & 3)) << 4) + (S::kWords == 1 ? q * 4 : (q & 1) * 8);
     // lanes whose token the tile does not have read another's: their columns are not stored
@@ -483,8 +488,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
                 for (int r = 0; r < RR; ++r) {
                   mz[r][0] = mz[r][1] = C::kMinusEight;
                   if (ZP) {
-                    mz[r][0] = mul2<T>((lds8(zp + r * 16) & 15u) * 0x00010001u, C::kNegate);
-                    mz[r][1] = mul2<T>((lds8(zp + r * 16 + 8) & 15u) * 0x00010001u, C::kNegate);
+                    mz[r][0] = mul2<T>((lds8(zp + loaded(r) * 16) & 15u) * 0x00010001u, C::kNegate);
+                    mz[r][1] = mul2<T>((lds8(zp + loaded(r) * 16 + 8) & 15u) * 0x00010001u, C::kNegate);
                   }
                 }
               }
@@ -525,14 +530,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
                 if (p.scale_f32) {
 #pragma unroll
                   for (int r = 0; r < RR; ++r) {
-                    scale[r][0] = __uint_as_float(lds32(sp + r * 64));
-                    scale[r][1] = __uint_as_float(lds32(sp + r * 64 + 32));
+                    scale[r][0] = __uint_as_float(lds32(sp + loaded(r) * 64));
+                    scale[r][1] = __uint_as_float(lds32(sp + loaded(r) * 64 + 32));
                   }
                 } else {
 #pragma unroll
                   for (int r = 0; r < RR; ++r) {
-                    scale[r][0] = scale_of(lds16(sp + r * 32), static_cast<T*>(nullptr));
-                    scale[r][1] = scale_of(lds16(sp + r * 32 + 16), static_cast<T*>(nullptr));
+                    scale[r][0] = scale_of(lds16(sp + loaded(r) * 32), static_cast<T*>(nullptr));
+                    scale[r][1] = scale_of(lds16(sp + loaded(r) * 32 + 16), static_cast<T*>(nullptr));
                   }
                 }
 #pragma unroll

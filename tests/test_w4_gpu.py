@@ -390,3 +390,15 @@ def test_an_out_that_requires_grad_is_refused(cuda_device):
     with torch.no_grad():
         assert fb.gemv_w4(x, w, s, out=out) is out
     assert torch.equal(out.detach(), fb.gemv_w4(x, w, s))
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("sdtype,M,N,K,G", [(torch.bfloat16, 2, 26304, 128, 128), (torch.bfloat16, 6, 53200, 256, 128),
+                                            (torch.float32, 1, 21568, 128, 128), (torch.float32, 5, 21568, 128, 128),
+                                            (torch.float32, 20, 41104, 128, 128), (torch.float32, 19, 43104, 1024, 256)])
+def test_parts_without_their_last_group(cuda_device, sdtype, M, N, K, G, zeros):
+    """Row parts one group short, one slice of K, and a stage that the boxes of scales fill to its
+    end: a load for the missing group past its box would leave the kernel's shared memory."""
+    w, s, z = weight((), N, K, G, zeros, sdtype, N + K, exact=True)
+    x = few_ones(M, K, N, torch.bfloat16)
+    assert torch.equal(fb.gemv_w4(*to(cuda_device, x, w, s, z)).cpu().double(), orc.product_ref(x, w, s, z)[0])
