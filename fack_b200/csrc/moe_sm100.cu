@@ -46,6 +46,12 @@ constexpr int kMaxDim = 1 << 20;
 
 constexpr int kSortRounds = 4;       // pairs per thread and chunk; their ranks stay in registers
 constexpr int kSortMaxBlocks = 128;
+// Shared memory of sort_place_kernel for `threads` threads; most, for 1024 experts and 1024 threads.
+constexpr size_t sort_smem_bytes(int threads, int E) {
+  return (E + 1) * sizeof(int) + static_cast<size_t>(threads / 32) * (E + 1) * sizeof(uint16_t);
+}
+constexpr int kSortSmemMost = static_cast<int>(sort_smem_bytes(1024, kMaxExperts));
+constexpr size_t kSortSmemPlain = 47 * 1024;   // beside the kernel's static arrays this needs no opt-in
 
 // Expert of pair p, or E when it is not routed here.  Ids are compared in
 // their own width, so a 64-bit id never aliases a small one.
@@ -618,11 +624,12 @@ static int sort_launch(const void* ids, int64_t pairs, int E, int* row_of, int* 
   const int64_t chunk = static_cast<int64_t>(threads) * kSortRounds;
   const int64_t share = ((pairs + blocks - 1) / blocks + chunk - 1) / chunk * chunk;
   const int64_t grid = (pairs + share - 1) / share;
-  const size_t smem = (E + 1) * sizeof(int) + static_cast<size_t>(threads / 32) * (E + 1) * sizeof(uint16_t);
-  // set on every call, so that each device has it: a host-side attribute, no device work
-  const cudaError_t e = smem > 48 * 1024 ? cudaFuncSetAttribute(sort_place_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                                static_cast<int>(smem))
-                                         : cudaSuccess;
+  const size_t smem = sort_smem_bytes(threads, E);
+  // Set on every call that needs it, so that each device has it (a host-side attribute, no device
+  // work), and always to the same value: it belongs to the function, whichever thread sorts what.
+  const cudaError_t e = smem > kSortSmemPlain ? cudaFuncSetAttribute(sort_place_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                                     kSortSmemMost)
+                                              : cudaSuccess;
   if (e != cudaSuccess) return fack::record_error(FACK_ERR_LAUNCH, cudaGetErrorString(e));
   if (grid > 1)
     sort_count_kernel<I><<<static_cast<unsigned>(grid), 1024, 0, s>>>(static_cast<const I*>(ids), pairs, share, E, hist);

@@ -444,3 +444,52 @@ def test_gradients_of_gradients_are_refused(cuda_device):
         first, = torch.autograd.grad(out, leaf, g, create_graph=True)
         with pytest.raises(RuntimeError):
             first.sum().backward()
+
+
+FRESH_SORT = """
+import torch
+import fack_b200 as fb
+from oracle.moe import sort_ref
+E, T, k = {E}, {T}, {k}
+ids = torch.randint(-1, E + 1, (T, k), generator=torch.Generator().manual_seed(E))
+for got, ref in zip(fb.moe_sort(ids.cuda(), E), sort_ref(ids, E)):
+    assert torch.equal(got.cpu(), ref)
+print("sorted")
+"""
+
+
+@pytest.mark.parametrize("E,T,k", [(844, 432, 8), (845, 1, 1), (846, 432, 8), (720, 2945, 1), (721, 3000, 2), (1024, 512, 8)])
+def test_sort_as_the_first_call_of_a_process(cuda_device, E, T, k):
+    """Shared memory just below and above what a kernel has without asking for more."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    run = subprocess.run([sys.executable, "-c", FRESH_SORT.format(E=E, T=T, k=k)],
+                         cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "sorted" in run.stdout, run.stdout + run.stderr
+
+
+def test_sorts_of_several_expert_counts_from_several_threads(cuda_device):
+    import threading
+    cases = []
+    for E in (725, 1024, 880, 64):
+        ids = torch.randint(-1, E + 1, (1500, 3), generator=torch.Generator().manual_seed(E))
+        cases.append((ids.to(cuda_device), E, orc.sort_ref(ids, E)))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(first):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for i in range(300):
+                ids, E, ref = cases[(first + i) % len(cases)]
+                try:
+                    plan = fb.moe_sort(ids, E)
+                    if i % 10 == 0 and not all(torch.equal(a.cpu(), b) for a, b in zip(plan, ref)):
+                        wrong.append((first, i))
+                except RuntimeError as e:
+                    wrong.append((first, i, str(e)))
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong, wrong[:3]
