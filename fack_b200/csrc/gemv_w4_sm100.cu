@@ -289,13 +289,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
       if (e < p.E) {
         first[i] = p.offsets[e];
         last[i] = p.offsets[e + 1];
-        bad |= first[i] < 0 || last[i] < first[i] || last[i] > p.rows;
+        bad |= (e == 0 ? first[i] != 0 : first[i] < 0) || last[i] < first[i] || last[i] > p.rows;
         if (last[i] > first[i]) tiles[i] = (last[i] - first[i] + p.tile - 1) / p.tile;
       }
       my_tiles += tiles[i];
       my_act += tiles[i] > 0;
     }
-    // offsets that do not ascend within the rows are no plan: nothing is routed
+    // offsets that do not ascend from 0 within the rows are no plan: nothing is routed
     if (__syncthreads_or(bad)) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) tiles[i] = 0;

@@ -523,7 +523,7 @@ int fack_moe_combine_bwd(const void* dout, int dtype, int64_t ldd, const void* y
  * fack_moe_sort plan.  With src, x is [T, K] and row r of y takes x's row
  * src[r] / topk (a src outside the pairs: a row of zeros); with src NULL, x is
  * [T*topk, K], sorted.  Rows behind offsets[E] are written as zeros (all rows,
- * where offsets do not ascend within 0..T*topk).
+ * where offsets do not ascend from 0 to at most T*topk).
  */
 int fack_gemv_w4(const void* x, int dtype, int64_t ldx, const void* w, const void* scales, int scale_dtype,
                  const void* zeros, int group, void* y, int64_t ldy, int M, int N, int K, void* stream);

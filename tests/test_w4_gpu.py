@@ -402,3 +402,16 @@ def test_parts_without_their_last_group(cuda_device, sdtype, M, N, K, G, zeros):
     w, s, z = weight((), N, K, G, zeros, sdtype, N + K, exact=True)
     x = few_ones(M, K, N, torch.bfloat16)
     assert torch.equal(fb.gemv_w4(*to(cuda_device, x, w, s, z)).cpu().double(), orc.product_ref(x, w, s, z)[0])
+
+
+def test_offsets_that_start_above_zero(cuda_device):
+    """Such offsets leave rows to no expert: nothing is routed, and every row is written."""
+    E, N, K = 3, 32, 64
+    w, s, _ = to(cuda_device, *weight((E,), N, K, 64, False, torch.float32, 1))
+    x = torch.ones((3, K), device=cuda_device, dtype=torch.bfloat16)
+    row_of = torch.arange(6, dtype=torch.int32, device=cuda_device).reshape(3, 2)
+    src = torch.arange(6, dtype=torch.int32, device=cuda_device)
+    for bad in ([2, 4, 6, 6], [6, 6, 6, 6], [1, 1, 1, 1], [-1, 2, 4, 6]):
+        plan = fb.MoePlan(row_of, src, torch.tensor(bad, dtype=torch.int32, device=cuda_device))
+        out = torch.full((6, N), float("nan"), device=cuda_device, dtype=torch.bfloat16)
+        assert (fb.gemv_w4_experts(x, w, s, plan, out=out) == 0).all()
