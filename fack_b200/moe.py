@@ -21,6 +21,7 @@ import ctypes
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import BLOCK, FP8
@@ -79,6 +80,14 @@ def _check_plan(plan, dev: torch.device):
     return T, topk, E
 
 
+def _refuse_tangent(t: torch.Tensor, name: str) -> None:
+    """No forward-mode derivative: a dual tensor does not require grad, and its
+    tangent would be lost without a word."""
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} has a forward-mode tangent, which this operator does not take; "
+                         "use its primal (torch.autograd.forward_ad.unpack_dual)")
+
+
 def _check_rows(t, name: str, rows: Optional[int] = None, width: Optional[int] = None, dtypes=DTYPES):
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 2:
         raise ValueError(f"{name} must be a 2-D CUDA tensor")
@@ -89,6 +98,7 @@ def _check_rows(t, name: str, rows: Optional[int] = None, width: Optional[int] =
                          f"got {tuple(t.shape)}")
     if t.shape[1] > 1 and t.stride(1) != 1 and t.shape[0]:
         raise ValueError(f"{name} must be contiguous along its rows")
+    _refuse_tangent(t, name)
 
 
 def _ld(t: torch.Tensor) -> int:
@@ -100,6 +110,7 @@ def _check_weights(weights, T, topk, dev):
     if not isinstance(weights, torch.Tensor) or weights.dtype != torch.float32 or tuple(weights.shape) != (T, topk) \
             or weights.device != dev:
         raise ValueError(f"weights must be a float32 [{T}, {topk}] tensor on {dev}")
+    _refuse_tangent(weights, "weights")
     return weights.contiguous()
 
 
@@ -258,10 +269,12 @@ class _Combine(torch.autograd.Function):
 def moe_gather(x: torch.Tensor, plan: MoePlan) -> torch.Tensor:
     """The tokens' rows in expert order: y [T*k, D] with y[r] = x[src[r] // k],
     zeros where a row has no pair.  ``x`` [T, D] fp32, bf16 or fp16, any row
-    stride.  Differentiable in x (:func:`moe_gather_backward`); inside a CUDA-graph
-    capture x may not be a leaf that requires grad."""
+    stride.  Differentiable in x in reverse mode (:func:`moe_gather_backward`;
+    a forward-mode tangent is refused); inside a CUDA-graph capture x may not be
+    a leaf that requires grad."""
     if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled() and isinstance(plan, MoePlan):
         _refuse_captured_leaf(x)
+        _refuse_tangent(x, "x")
         return _Gather.apply(x, plan)
     return _gather(x, plan)
 
@@ -271,14 +284,16 @@ def moe_combine(y: torch.Tensor, weights: torch.Tensor, plan: MoePlan) -> torch.
     y[row_of[t, j]] over the pairs that have a row, in fp32, slots in order,
     rounded once to y's type.  ``y`` [T*k, D] fp32, bf16 or fp16, any row
     stride; ``weights`` fp32 [T, k].  Differentiable in both
-    (:func:`moe_combine_backward`); inside a CUDA-graph capture neither may be a
-    leaf that requires grad."""
+    in reverse mode (:func:`moe_combine_backward`; a forward-mode tangent is
+    refused); inside a CUDA-graph capture neither may be a leaf that requires grad."""
     if weights is None:
         raise ValueError("weights must be a float32 [T, k] tensor")
     if torch.is_grad_enabled() and isinstance(plan, MoePlan) and (getattr(y, "requires_grad", False)
                                                                   or getattr(weights, "requires_grad", False)):
         if isinstance(y, torch.Tensor) and isinstance(weights, torch.Tensor):
             _refuse_captured_leaf(y, weights)
+            _refuse_tangent(y, "y")
+            _refuse_tangent(weights, "weights")
         return _Combine.apply(y, weights, plan)
     return _combine(y, weights, plan)
 

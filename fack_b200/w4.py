@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .moe import DTYPES, MoePlan, _call, _check_plan, _check_rows, _ld
+from .moe import DTYPES, MoePlan, _call, _check_plan, _check_rows, _ld, _refuse_tangent
 
 TYPES = (torch.bfloat16, torch.float16)
 
@@ -47,6 +47,7 @@ def _check_weight(x, w, scales, zeros, lead: tuple):
                          f"(N = {N}, group = {G})")
     if (x.requires_grad or scales.requires_grad) and torch.is_grad_enabled():
         raise ValueError("4-bit products have no gradient; detach the operands or call under torch.no_grad()")
+    _refuse_tangent(scales, "scales")
     return N, K, G
 
 
@@ -58,6 +59,7 @@ def _check_out(out, rows: int, N: int, x):
         raise ValueError(f"out must be a {x.dtype} [{rows}, {N}] tensor with unit column stride on {x.device}")
     if out.requires_grad and torch.is_grad_enabled():
         raise ValueError("out is written outside autograd: it must not require grad")
+    _refuse_tangent(out, "out")
     return out
 
 

@@ -493,3 +493,26 @@ def test_sorts_of_several_expert_counts_from_several_threads(cuda_device):
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not wrong, wrong[:3]
+
+
+def test_forward_mode_is_refused(cuda_device):
+    """A dual tensor does not require grad: without a check its tangent would be dropped."""
+    import torch.autograd.forward_ad as fwd
+    plan = fb.moe_sort(torch.tensor([[0, 1], [1, 2], [0, 2]], device=cuda_device), 3)
+    x, y = torch.randn((3, 128), device=cuda_device), torch.randn((6, 128), device=cuda_device)
+    w = torch.rand((3, 2), device=cuda_device)
+    codes = torch.randint(0, 256, (32, 64), device=cuda_device, dtype=torch.uint8)
+    s = torch.ones((1, 32), device=cuda_device)
+    xb = x.bfloat16()
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for f in (lambda: fb.moe_gather(dual(x), plan), lambda: fb.moe_combine(dual(y), w, plan),
+                  lambda: fb.moe_combine(y, dual(w), plan), lambda: fb.moe_gather_quant(dual(x), plan),
+                  lambda: fb.moe_gather_backward(dual(y), plan), lambda: fb.moe_combine_backward(dual(x), y, w, plan),
+                  lambda: fb.moe_combine_backward(x, dual(y), w, plan), lambda: fb.moe_combine_backward(x, y, dual(w), plan),
+                  lambda: fb.moe_gather(dual(x).requires_grad_(), plan),
+                  lambda: fb.gemv_w4(dual(xb), codes, s), lambda: fb.gemv_w4(xb, codes, dual(s)),
+                  lambda: fb.gemv_w4(xb, codes, s, out=dual(torch.zeros((3, 32), device=cuda_device).bfloat16()))):
+            with pytest.raises(ValueError, match="forward"):
+                f()
+        assert torch.equal(fb.moe_gather(x, plan), x[plan.src.long() // 2])
