@@ -786,7 +786,7 @@ int fack_moe_gather_quant(const void* x, int dtype, int64_t ldx, int T, int topk
   if (K < kBlk || K % kBlk || K > kMaxDim) return FACK_ERR_BAD_SHAPE;
   if (dtype != FACK_DTYPE_F32 && dtype != FACK_DTYPE_BF16) return FACK_ERR_BAD_ARG;
   if (!x || !xq || !x_scale || !aligned(x, 16) || !aligned(xq, 16) || !aligned(x_scale, 4)) return FACK_ERR_BAD_ALIGN;
-  if (ldx < 0 || ldx % 8 || ldq < K || ldq % 16 || lds < K / kBlk) return FACK_ERR_BAD_STRIDE;
+  if (ldx < 0 || ldx * elem_size(dtype) % 16 || ldq < K || ldq % 16 || lds < K / kBlk) return FACK_ERR_BAD_STRIDE;
   int sms = 0;
   st = fack::sm100_device(&sms);
   if (st != FACK_OK) return st;

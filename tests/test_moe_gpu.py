@@ -516,3 +516,13 @@ def test_forward_mode_is_refused(cuda_device):
             with pytest.raises(ValueError, match="forward"):
                 f()
         assert torch.equal(fb.moe_gather(x, plan), x[plan.src.long() // 2])
+
+
+def test_quant_fp32_rows_of_any_16_byte_stride(cuda_device):
+    """The kernel reads 16 bytes at a time: strides of 4, 8 and 12 elements modulo 16."""
+    plan = fb.moe_sort(torch.tensor([[0, 1], [1, 2], [0, 2]], device=cuda_device), 3)
+    wide = torch.randn((3, 272), device=cuda_device)
+    for off, ld in ((0, 260), (4, 264), (8, 268), (0, 272)):
+        x = wide.as_strided((3, 256), (ld, 1), off)
+        for a, b in zip(fb.moe_gather_quant(x, plan), fb.moe_gather_quant(x.contiguous(), plan)):
+            assert torch.equal(a.float(), b.float())

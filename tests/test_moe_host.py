@@ -105,3 +105,10 @@ def test_plan_checks():
                 plan._replace(row_of=plan.row_of.reshape(-1)), plan._replace(offsets=None), tuple(plan), None):
         with pytest.raises(ValueError):
             moe._check_plan(bad, cpu)
+
+
+def test_quant_rows_of_every_type_are_16_byte_strides():
+    """fp32 strides are multiples of 4 elements, bf16 ones of 8."""
+    for dtype, bad in ((0, (257, 258, 262)), (1, (257, 260, 268))):
+        for ldx in bad:
+            assert call("fack_moe_gather_quant", dtype=dtype, ldx=ldx) == BAD_STRIDE
