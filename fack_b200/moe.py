@@ -303,8 +303,11 @@ def moe_gather_quant(x: torch.Tensor, plan: MoePlan):
     pass: (xq e4m3 [T*k, K], x_scale fp32 [T*k, K/128]), the sorted rows' codes
     and logical scales as :func:`fack_b200.gemm_blockscale` takes them per
     expert.  ``x`` [T, K] fp32 or bf16, K % 128 == 0, rows 16-byte aligned.
-    Rows without a pair have zero codes and scale 1; a 128-wide group that
-    holds NaN has scale and codes NaN.  Not differentiable."""
+    Rows without a pair have zero codes and scale 1.  NaN in a 128-wide group makes
+    its scale and codes NaN; an infinity makes its scale infinite, the infinities
+    NaN codes and the rest zero codes; an amax that is too small for a scale makes
+    it 1 and the codes zero (quantize_activations: NaN left out of the amax, -240
+    for NaN quotients, scale 0).  Not differentiable."""
     _check_rows(x, "x", dtypes=(torch.float32, torch.bfloat16))
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("moe_gather_quant has no gradient; detach x or call it under torch.no_grad()")

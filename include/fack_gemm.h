@@ -477,8 +477,14 @@ int fack_gemm_tn(int kind, const void* a, int64_t lda, const void* b, int b_pack
  *                          per-128 scales of x[t] (fp32 or bf16; K % 128 == 0,
  *                          16-byte aligned rows): scale = amax/240, 1 where that
  *                          is 0, codes e4m3fn(clamp(x/scale, -240, 240)), the
- *                          values of fack_quant_act; a group that holds NaN
- *                          gets scale and codes NaN
+ *                          values of fack_quant_act where the group is finite
+ *                          and amax/240 does not round to 0, or all zero.
+ *                          Else: NaN in a group makes its scale and codes NaN;
+ *                          an infinity makes its scale infinite, the infinities
+ *                          NaN codes and the rest zero codes; an amax too small
+ *                          for a scale makes it 1 and the codes zero.
+ *                          (fack_quant_act leaves NaN out of amax, has -240 for
+ *                          NaN quotients, and scale 0 with +-240 for the last.)
  *   fack_moe_combine       out[t] = sum_j weights[t, j] * y[row_of[t, j]] over the
  *                          pairs with a row, in fp32 in the order of j, rounded
  *                          once; weights fp32 [T, topk] contiguous, NULL for

@@ -526,3 +526,33 @@ def test_quant_fp32_rows_of_any_16_byte_stride(cuda_device):
         x = wide.as_strided((3, 256), (ld, 1), off)
         for a, b in zip(fb.moe_gather_quant(x, plan), fb.moe_gather_quant(x.contiguous(), plan)):
             assert torch.equal(a.float(), b.float())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gather_quant_beside_the_quantiser_on_what_is_not_finite(cuda_device, dtype):
+    """Equal where a group is finite with a scale above 0 or all zero; what the two do with the rest."""
+    T, K, inf, nan = 10, 384, float("inf"), float("nan")
+    plan = fb.moe_sort(torch.zeros((T, 1), dtype=torch.int32, device=cuda_device), 1)
+    x = torch.randn((T, K), generator=torch.Generator().manual_seed(1))
+    for t, k, v in ((0, 3, nan), (1, 130, inf), (2, 131, -inf), (3, 5, inf), (3, 6, nan), (4, 0, inf), (4, 127, -inf),
+                    (5, 383, nan)):
+        x[t, k] = v
+    x[6, 128:256] = 0
+    x[7, :128] = 1e-40                                  # both types hold about this; the scale is about 4e-43
+    x[8, :128] = 2.0 ** -149 if dtype == torch.float32 else 1.0
+    x = x.to(dtype)
+    group = x.float().view(T, -1, 128)
+    xq, xs = (t.float().cpu() for t in fb.moe_gather_quant(x.to(cuda_device), plan))
+    q, s = (t.float().cpu() for t in fb.quantize_activations(x.to(cuda_device), layout="logical"))
+    xq, q = xq.view_as(group), q.view_as(group)
+    has_nan, has_inf = group.isnan().any(2), group.isinf().any(2)
+    tiny = (group.abs().amax(2) > 0) & (group.abs().amax(2) / 240.0 == 0)
+    same = ~(has_nan | has_inf | tiny)
+    assert torch.equal(xs[same], s[same]) and torch.equal(xq[same], q[same])
+    assert xs[has_nan].isnan().all() and xq[has_nan].isnan().all() and not s[has_nan].isnan().any()
+    only = has_inf & ~has_nan
+    assert xs[only].isinf().all() and s[only].isinf().all()
+    assert torch.equal(xq[only].isnan(), group[only].isinf()) and (xq[only].nan_to_num(0.0) == 0).all()
+    assert torch.equal(q[only], torch.where(group[only].isinf(), -240.0, 0.0))
+    assert (xs[tiny] == 1).all() and (xq[tiny] == 0).all() and (s[tiny] == 0).all() and (q[tiny] == 240).all()
+    assert int(tiny.sum()) == (1 if dtype == torch.float32 else 0)
