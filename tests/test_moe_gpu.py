@@ -556,3 +556,22 @@ def test_gather_quant_beside_the_quantiser_on_what_is_not_finite(cuda_device, dt
     assert torch.equal(q[only], torch.where(group[only].isinf(), -240.0, 0.0))
     assert (xs[tiny] == 1).all() and (xq[tiny] == 0).all() and (s[tiny] == 0).all() and (q[tiny] == 240).all()
     assert int(tiny.sum()) == (1 if dtype == torch.float32 else 0)
+
+
+def test_gather_quant_codes_on_midpoints(cuda_device):
+    """bf16 values that lie between two codes exactly, with scales that are no powers of two: the
+    definition divides by 240 and by the scale, and a product with a rounded reciprocal would
+    take some of them the other way."""
+    g = torch.Generator().manual_seed(3)
+    T, K = 64, 7168
+    x = torch.randn((T, K), generator=g)
+    x = torch.where(torch.rand((T, K), generator=g) < 1e-3, x * 50, x).bfloat16()
+    group = x.float().view(T, -1, 128)
+    scale = group.abs().amax(2, keepdim=True) / 240.0
+    other = group.abs().amax(2, keepdim=True) * torch.tensor(1.0 / 240.0)
+    by = lambda s: (group / s).clamp(-240, 240).to(torch.float8_e4m3fn).float()  # noqa: E731
+    assert (by(scale) != by(other)).sum() > 500               # such values are among them
+    plan = fb.moe_sort(torch.arange(T, device=cuda_device)[:, None] % 5, 5)
+    xq, xs = fb.moe_gather_quant(x.to(cuda_device), plan)
+    rows = plan.src.cpu().long()
+    assert torch.equal(xs.cpu(), scale[rows, :, 0]) and torch.equal(xq.float().cpu(), by(scale).view(T, K)[rows])
