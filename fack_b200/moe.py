@@ -229,7 +229,9 @@ def _grad_rows(g: torch.Tensor) -> torch.Tensor:
 def _refuse_captured_leaf(*inputs) -> None:
     """No gradient of a leaf inside a CUDA-graph capture: where an eager graph of
     the same leaf is alive, autograd would make the capture wait on that graph's
-    stream, which ends the process.  The backward functions have no such state."""
+    stream, which ends the process.  The backward functions have no such state.
+    Whether such a graph lives cannot be asked; where none does (the static inputs of
+    torch.cuda.make_graphed_callables), a view of the leaf is taken."""
     for t in inputs:
         if t.requires_grad and t.is_leaf and t.is_cuda and torch.cuda.is_current_stream_capturing():
             raise ValueError("a captured gather or combine takes no leaf that requires grad; call "

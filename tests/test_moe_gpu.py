@@ -575,3 +575,28 @@ def test_gather_quant_codes_on_midpoints(cuda_device):
     xq, xs = fb.moe_gather_quant(x.to(cuda_device), plan)
     rows = plan.src.cpu().long()
     assert torch.equal(xs.cpu(), scale[rows, :, 0]) and torch.equal(xq.float().cpu(), by(scale).view(T, K)[rows])
+
+
+def test_a_graphed_callable(cuda_device):
+    """torch.cuda.make_graphed_callables: its static inputs are leaves, taken through a view;
+    outputs and gradients equal those of the eager layer, for new inputs too."""
+    T, k, E, D = 70, 3, 8, 96
+    plan = gpu_plan(T, k, E, 6, cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(7)
+    rand = lambda *s: torch.randn(s, generator=g, device=cuda_device)  # noqa: E731
+
+    def layer(x, w):
+        y = fb.moe_gather(x.view_as(x), plan)
+        return fb.moe_combine(y * 3, w.view_as(w), plan)
+
+    x, w = rand(T, D).requires_grad_(), rand(T, k).requires_grad_()
+    graphed = torch.cuda.make_graphed_callables(layer, (x, w))
+    for _ in range(3):
+        a, b, dout = rand(T, D), rand(T, k), rand(T, D)
+        got, ref = [], []
+        for f, out in ((graphed, got), (layer, ref)):
+            xa, wb = a.clone().requires_grad_(), b.clone().requires_grad_()
+            y = f(xa, wb)
+            out += [y.detach().clone(), *(t.clone() for t in torch.autograd.grad(y, (xa, wb), dout))]
+        for p, q in zip(got, ref):
+            assert torch.equal(p, q)
