@@ -83,6 +83,7 @@ SIGNATURES = {
     "fack_moe_combine": (_c_int, [_c_p, _c_int, _c_i64, _c_p, _c_int, _c_int, _c_int, _c_p, _c_p, _c_i64, _c_p]),
     "fack_moe_combine_bwd": (_c_int, [_c_p, _c_int, _c_i64, _c_p, _c_i64, _c_p, _c_int, _c_int, _c_int, _c_p, _c_p,
                                       _c_int, _c_p, _c_i64, _c_p, _c_p]),
+    "fack_gemv_w4_plan": (_c_int, [_c_int] * 6 + [ctypes.POINTER(_c_int)] * 4),
     "fack_gemv_w4": (_c_int, [_c_p, _c_int, _c_i64, _c_p, _c_p, _c_int, _c_p, _c_int, _c_p, _c_i64, _c_int, _c_int,
                               _c_int, _c_p]),
     "fack_gemv_w4_experts": (_c_int, [_c_p, _c_int, _c_i64, _c_p, _c_p, _c_int, _c_p, _c_int, _c_p, _c_p, _c_int,

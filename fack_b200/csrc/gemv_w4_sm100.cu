@@ -749,13 +749,13 @@ static double expected_tiles(int T, int topk, int E, int tile) {
 
 // Tokens per tile (8 NT at most) and the plan.  An expert's rows are known on the
 // device alone; it is not likely to have more than there are tokens, and one token has topk.
-static void choose(Args& a, int tokens, int sms, int* NT, int* R) {
+static void choose(Args& a, bool experts, int tokens, int sms, int* NT, int* R) {
   Plan p[2];
   int tile[2];
   for (int i = 0; i < 2; ++i) {
     const int most = 8 * (i + 1);
     double tiles;
-    if (a.offsets) {
+    if (experts) {
       tile[i] = tokens < most ? tokens : most;
       tiles = expected_tiles(tokens, a.topk, a.E, tile[i]);
     } else {
@@ -763,7 +763,7 @@ static void choose(Args& a, int tokens, int sms, int* NT, int* R) {
       tile[i] = static_cast<int>((a.rows + n - 1) / n);      // evenly filled
       tiles = static_cast<double>(n);
     }
-    p[i] = plan(i + 1, tiles, a.offsets != nullptr && tokens > 1, a.N, a.K, a.G, sms);
+    p[i] = plan(i + 1, tiles, experts && tokens > 1, a.N, a.K, a.G, sms);
   }
   const int i = tile[1] > 8 && p[1].us < p[0].us;
   *NT = i + 1;
@@ -773,9 +773,15 @@ static void choose(Args& a, int tokens, int sms, int* NT, int* R) {
   a.groups = p[i].groups;
 }
 
-static int run(Args& a, int dtype, int scale_dtype, int tokens, void* stream) {
+static int check_shape(const Args& a) {
   if (a.rows < 1 || a.N < 16 || a.N % 16 || a.N > (1 << 24) || a.K < 32 || a.K > (1 << 20)) return FACK_ERR_BAD_SHAPE;
   if ((a.G != 32 && a.G != 64 && (a.G < 128 || a.G % 128)) || a.K % a.G) return FACK_ERR_BAD_ARG;
+  return FACK_OK;
+}
+
+static int run(Args& a, int dtype, int scale_dtype, int tokens, void* stream) {
+  int st = check_shape(a);
+  if (st != FACK_OK) return st;
   if (dtype != FACK_DTYPE_BF16 && dtype != FACK_DTYPE_F16) return FACK_ERR_BAD_ARG;
   if (scale_dtype != FACK_DTYPE_F32 && scale_dtype != dtype) return FACK_ERR_BAD_ARG;
   if (!a.x || !a.w || !a.scales || !a.y || !aligned(a.x, 16) || !aligned(a.w, 16) || !aligned(a.scales, 16) ||
@@ -783,7 +789,7 @@ static int run(Args& a, int dtype, int scale_dtype, int tokens, void* stream) {
     return FACK_ERR_BAD_ALIGN;
   if (a.ldx < 0 || a.ldx % 8 || a.ldy < a.N) return FACK_ERR_BAD_STRIDE;
   int sms = 0;
-  const int st = sm100_device(&sms);
+  st = sm100_device(&sms);
   if (st != FACK_OK) return st;
   a.scale_f32 = scale_dtype == FACK_DTYPE_F32;
   a.status = device_status_word();
@@ -793,7 +799,7 @@ static int run(Args& a, int dtype, int scale_dtype, int tokens, void* stream) {
   if (static_cast<int64_t>(a.E) * a.N > INT32_MAX - 1024 || static_cast<int64_t>(a.E) * (a.K / a.G) > INT32_MAX - 1024)
     return FACK_ERR_BAD_SHAPE;
   int NT, R;
-  choose(a, tokens, sms, &NT, &R);
+  choose(a, a.offsets != nullptr, tokens, sms, &NT, &R);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == FACK_DTYPE_BF16)
     return a.zeros ? by_group<__nv_bfloat16, true>(a, NT, R, sms, s) : by_group<__nv_bfloat16, false>(a, NT, R, sms, s);
@@ -803,6 +809,34 @@ static int run(Args& a, int dtype, int scale_dtype, int tokens, void* stream) {
 }  // namespace fack_w4
 
 extern "C" {
+
+int fack_gemv_w4_plan(int tokens, int topk, int num_experts, int N, int K, int group, int* tile, int* warp_groups, int* split,
+                      int* item_groups) {
+  using namespace fack_w4;
+  Args a = {};
+  const bool experts = topk != 0 || num_experts != 0;
+  if (tokens < 1 || (experts && (topk < 1 || topk > kMaxTopk || num_experts < 1 || num_experts > kMaxExperts ||
+                                 static_cast<int64_t>(tokens) * topk > INT32_MAX)))
+    return FACK_ERR_BAD_SHAPE;
+  a.topk = experts ? topk : 1;
+  a.E = experts ? num_experts : 1;
+  a.rows = tokens * a.topk;
+  a.N = N;
+  a.K = K;
+  a.G = group;
+  int st = check_shape(a);
+  if (st != FACK_OK) return st;
+  if (!tile || !warp_groups || !split || !item_groups) return FACK_ERR_BAD_ARG;
+  int sms = 0;
+  st = sm100_device(&sms);
+  if (st != FACK_OK) return st;
+  int NT;
+  choose(a, experts, tokens, sms, &NT, warp_groups);
+  *tile = a.tile;
+  *split = a.split;
+  *item_groups = a.groups;
+  return FACK_OK;
+}
 
 int fack_gemv_w4(const void* x, int dtype, int64_t ldx, const void* w, const void* scales, int scale_dtype,
                  const void* zeros, int group, void* y, int64_t ldy, int M, int N, int K, void* stream) {

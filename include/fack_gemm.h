@@ -531,6 +531,11 @@ int fack_moe_combine_bwd(const void* dout, int dtype, int64_t ldd, const void* y
  * [T*topk, K], sorted.  Rows behind offsets[E] are written as zeros (all rows,
  * where offsets do not ascend from 0 to at most T*topk).
  */
+/* The plan of a call on the current device (topk = num_experts = 0: fack_gemv_w4 with
+ * M = tokens): at most `tile` tokens at a time (one MMA's eight, or two's), warp_groups
+ * 16-row groups a warp, `split` slices of K among a CTA's warps, item_groups groups an item. */
+int fack_gemv_w4_plan(int tokens, int topk, int num_experts, int N, int K, int group, int* tile, int* warp_groups, int* split,
+                      int* item_groups);
 int fack_gemv_w4(const void* x, int dtype, int64_t ldx, const void* w, const void* scales, int scale_dtype,
                  const void* zeros, int group, void* y, int64_t ldy, int M, int N, int K, void* stream);
 int fack_gemv_w4_experts(const void* x, int dtype, int64_t ldx, const void* w, const void* scales, int scale_dtype,

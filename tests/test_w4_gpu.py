@@ -415,3 +415,68 @@ def test_offsets_that_start_above_zero(cuda_device):
         plan = fb.MoePlan(row_of, src, torch.tensor(bad, dtype=torch.int32, device=cuda_device))
         out = torch.full((6, N), float("nan"), device=cuda_device, dtype=torch.bfloat16)
         assert (fb.gemv_w4_experts(x, w, s, plan, out=out) == 0).all()
+
+
+def plan_of(tokens, N, K, G, topk=0, experts=0):
+    """(tokens a tile, groups a warp, slices of K, groups an item) of a call."""
+    import ctypes
+    from fack_b200 import _lib
+    out = [ctypes.c_int() for _ in range(4)]
+    assert _lib.load().fack_gemv_w4_plan(tokens, topk, experts, N, K, G, *map(ctypes.byref, out)) == 0
+    return tuple(v.value for v in out)
+
+
+LARGE_K = {32: 416, 64: 448, 128: 384, 256: 512}       # three or four blocks of 128; those of 32 and 64 end inside one
+# tokens and rows of layers whose warps take four groups of 16 rows: with 8 and 16 tokens a tile, items of one
+# box and of two, full and with parts a group short
+LARGE = [(21, 5936), (40, 3152), (40, 28336), (40, 25104), (40, 5504), (40, 3936), (40, 23536), (40, 15120)]
+LARGE_EXPERTS = [(33, 4, 4, 896), (33, 2, 2, 1504), (150, 2, 2, 3472), (150, 4, 4, 1840), (150, 4, 4, 352), (150, 2, 2, 512),
+                 (150, 2, 2, 2944), (150, 2, 2, 1952)]
+
+
+@pytest.mark.parametrize("G", [32, 64, 128, 256])
+def test_the_large_layers_take_every_form_of_four_groups_a_warp(cuda_device, G):
+    def form(p):
+        tile, groups, split, item = p
+        return groups, tile > 8, item > 16, item < groups * 8 // split
+
+    want = {(4, two, boxes, part) for two in (False, True) for boxes in (False, True) for part in (False, True)}
+    assert {form(plan_of(M, N, LARGE_K[G], G)) for M, N in LARGE} == want
+    assert {form(plan_of(T, N, LARGE_K[G], G, k, E)) for T, k, E, N in LARGE_EXPERTS} == want
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("G", [32, 64, 128, 256])
+@pytest.mark.parametrize("M,N", LARGE)
+def test_exact_with_four_groups_a_warp(cuda_device, M, N, G, zeros):
+    K, dtype = LARGE_K[G], TYPES[(M + N // 16 + zeros) % 2]
+    w, s, z = weight((), N, K, G, zeros, torch.float32 if N % 32 else dtype, N + G, exact=True)
+    x = few_ones(M, K, N, dtype)
+    assert torch.equal(fb.gemv_w4(*to(cuda_device, x, w, s, z)).cpu().double(), orc.product_ref(x, w, s, z)[0])
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("G", [32, 64, 128, 256])
+@pytest.mark.parametrize("T,k,E,N", LARGE_EXPERTS)
+def test_experts_with_four_groups_a_warp(cuda_device, T, k, E, N, G, zeros):
+    K, dtype = LARGE_K[G], TYPES[(T + N // 16 + zeros) % 2]
+    w, s, z = weight((E,), N, K, G, zeros, dtype if N % 32 else torch.float32, N + G, exact=True)
+    ids, x = make_ids(T, k, E, N, "any"), few_ones(T, K, N, dtype)
+    row_of, src, offsets = moe_orc.sort_ref(ids, E)
+    ref = orc.experts_ref(moe_orc.gather_ref(x, src, k), w, s, z, offsets, T * k)[0]
+    plan = fb.moe_sort(ids.to(cuda_device), E)
+    xd, wd, sd, zd = to(cuda_device, x, w, s, z)
+    assert torch.equal(fb.gemv_w4_experts(xd, wd, sd, plan, zd).cpu().double(), ref)
+    rows = fb.moe_gather(xd, plan)
+    assert torch.equal(fb.gemv_w4_experts(rows, wd, sd, plan, zd, sorted_rows=True).cpu().double(), ref)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("M,N,K,G", [(1, 37888, 1344, 32), (3, 33344, 1344, 64), (8, 65536, 2048, 128), (2, 57344, 1024, 256),
+                                     (13, 65536, 704, 64), (11, 57344, 672, 32)])
+def test_exact_in_wide_layers(cuda_device, M, N, K, G, zeros):
+    w, s, z = weight((), N, K, G, zeros, torch.bfloat16, N + G, exact=True)
+    x = few_ones(M, K, N, torch.bfloat16)
+    tile, groups, split, item = plan_of(M, N, K, G)
+    assert tile == M and groups == 4
+    assert torch.equal(fb.gemv_w4(*to(cuda_device, x, w, s, z)).cpu().double(), orc.product_ref(x, w, s, z)[0])

@@ -83,3 +83,15 @@ def test_weight_checks():
             _check_weight(*bad)
     with torch.no_grad():
         assert _check_weight(x.clone().requires_grad_(), w, s, z, ()) == (64, 256, 128)
+
+
+@pytest.mark.parametrize("args,status", [
+    ((0, 0, 0, 64, 256, 128), BAD_SHAPE), ((4, 2, 0, 64, 256, 128), BAD_SHAPE), ((4, 0, 8, 64, 256, 128), BAD_SHAPE),
+    ((4, 65, 8, 64, 256, 128), BAD_SHAPE), ((4, 2, 1025, 64, 256, 128), BAD_SHAPE), ((1 << 30, 2, 8, 64, 256, 128), BAD_SHAPE),
+    ((4, 0, 0, 72, 256, 128), BAD_SHAPE), ((4, 0, 0, 64, 0, 128), BAD_SHAPE), ((4, 0, 0, 64, 256, 96), BAD_ARG),
+    ((4, 0, 0, 64, 320, 128), BAD_ARG)])
+def test_plan_refusals(args, status):
+    import ctypes
+    out = [ctypes.c_int() for _ in range(4)]
+    assert _lib.load().fack_gemv_w4_plan(*args, *map(ctypes.byref, out)) == status
+    assert _lib.load().fack_gemv_w4_plan(4, 0, 0, 64, 256, 128, None, *map(ctypes.byref, out[1:])) == BAD_ARG
