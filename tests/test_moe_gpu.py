@@ -600,3 +600,57 @@ def test_a_graphed_callable(cuda_device):
             out += [y.detach().clone(), *(t.clone() for t in torch.autograd.grad(y, (xa, wb), dout))]
         for p, q in zip(got, ref):
             assert torch.equal(p, q)
+
+
+# rows wide enough for two places a thread, tokens enough for a block each: the second place whole, partly
+# filled and (fp32) with several rounds; one and two, three and four slots, and five, which take one place
+TWO_PLACES = [(300, 1, 7, 1024), (300, 2, 9, 1032), (301, 2, 9, 7168), (297, 2, 5, 4104), (301, 3, 6, 2056),
+              (333, 4, 8, 4104), (299, 4, 12, 1024), (298, 5, 9, 2056)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,k,E,D", TWO_PLACES)
+def test_two_places_of_a_row_at_once(cuda_device, dtype, T, k, E, D):
+    plan = gpu_plan(T, k, E, D + T, cuda_device)
+    g = torch.Generator().manual_seed(T + D)
+    y, dout = torch.randn((T * k, D), generator=g).to(dtype), torch.randn((T, D), generator=g).to(dtype)
+    w = torch.randn((T, k), generator=g)
+    y[int(plan.offsets[-1]):] = float("nan")
+    yd, dd, wd = y.to(cuda_device), dout.to(cuda_device), w.to(cuda_device)
+    ref, mag = orc.combine_ref(y, w, plan.row_of)
+    close(fb.moe_combine(yd, wd, plan), ref, k * U32 * mag + rounding(dtype, ref))
+    ref, mag = orc.combine_ref(y, None, plan.row_of)
+    close(fb.moe_gather_backward(yd, plan), ref, k * U32 * mag + rounding(dtype, ref))
+    rdy, rdw, mag = orc.combine_bwd_ref(dout, y, w, plan.row_of)
+    dy, dw = fb.moe_combine_backward(dd, yd, wd, plan)
+    close(dy, rdy, U32 * rdy.abs() + rounding(dtype, rdy))
+    close(dw, rdw, D * U32 * mag)
+    assert torch.equal(fb.moe_combine_backward(dd, None, wd, plan, need_dweights=False)[0], dy)
+    assert torch.equal(fb.moe_combine_backward(dd, yd, wd, plan, need_dy=False)[1], dw)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_of_a_plan_with_entries_out_of_range(cuda_device, dtype):
+    """No row lies behind the last one, so nothing but the valid entries writes."""
+    T, k, D = 6, 2, 128
+    row_of = torch.tensor([[0, 1], [2 ** 31 - 1, 3], [-5, 12], [-2 ** 31, 5], [99, 7], [8, 9]], dtype=torch.int32)
+    valid = (row_of >= 0) & (row_of < T * k)
+    plan = fb.MoePlan(*(t.to(cuda_device) for t in (row_of, torch.zeros(T * k, dtype=torch.int32),
+                                                    torch.tensor([0, T * k], dtype=torch.int32))))
+    g = torch.Generator().manual_seed(1)
+    x, y = torch.randn((T, D), generator=g).to(dtype), torch.randn((T * k, D), generator=g).to(dtype)
+    w = torch.rand((T, k), generator=g)
+    got = fb.moe_gather(x.to(cuda_device), plan).cpu()
+    dy, dw = (t.cpu() for t in fb.moe_combine_backward(*(t.to(cuda_device) for t in (x, y, w)), plan))
+    quant = None if dtype == torch.float16 else [t.cpu() for t in fb.moe_gather_quant(x.to(cuda_device), plan)]
+    whole = None if dtype == torch.float16 else [t.cpu() for t in fb.quantize_activations(x.to(cuda_device), layout="logical")]
+    _, rdw, mag = orc.combine_bwd_ref(x, y, w, torch.where(valid, row_of, -1))
+    close(dw, rdw, D * U32 * mag)
+    assert (dw[~valid] == 0).all()
+    for t, j in valid.nonzero().tolist():
+        r = int(row_of[t, j])
+        want = w[t, j].double() * x[t].double()
+        assert torch.equal(got[r], x[t])
+        close(dy[r], want, U32 * want.abs() + rounding(dtype, want))
+        if quant:
+            assert torch.equal(quant[0][r].view(torch.uint8), whole[0][t].view(torch.uint8)) and torch.equal(quant[1][r], whole[1][t])
