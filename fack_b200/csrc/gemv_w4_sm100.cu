@@ -738,8 +738,9 @@ static int by_group(Args& a, int NT, int R, int sms, cudaStream_t s) {
 static double expected_tiles(int T, int topk, int E, int tile) {
   const double q = static_cast<double>(topk) / E, mean = q * T;
   if (q >= 1.0) return static_cast<double>(E) * ((static_cast<int64_t>(T) * topk / E + tile - 1) / tile);
-  if (mean > 200.0) return E * (mean / tile + 0.5);
-  double sum = 0.0, p = exp(T * log1p(-q));
+  const double none = T * log1p(-q);            // logarithm of the chance that no token takes an expert
+  if (mean > 200.0 || none < -700.0) return E * (mean / tile + 0.5);
+  double sum = 0.0, p = exp(none);
   for (int x = 1; x <= T && x < 600; ++x) {
     p *= static_cast<double>(T - x + 1) / x * q / (1.0 - q);
     sum += p * ((x + tile - 1) / tile);

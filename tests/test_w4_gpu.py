@@ -480,3 +480,13 @@ def test_exact_in_wide_layers(cuda_device, M, N, K, G, zeros):
     tile, groups, split, item = plan_of(M, N, K, G)
     assert tile == M and groups == 4
     assert torch.equal(fb.gemv_w4(*to(cuda_device, x, w, s, z)).cpu().double(), orc.product_ref(x, w, s, z)[0])
+
+
+def test_the_plan_of_nearly_all_experts(cuda_device):
+    """63 of 64 experts a token: the chance that an expert has no row is below what a double holds
+    from 180 tokens on; the plan is that of one token less or of all experts, not one for no rows."""
+    for N, K in ((4096, 2048), (7168, 512)):
+        want = plan_of(150, N, K, 128, 63, 64)
+        assert want[0] == 16
+        for T in (170, 171, 180, 200, 203, 204, 260):
+            assert plan_of(T, N, K, 128, 63, 64)[:2] == want[:2] == plan_of(T, N, K, 128, 64, 64)[:2]
