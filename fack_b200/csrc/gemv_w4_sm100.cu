@@ -24,11 +24,13 @@
 //     of (expert, row tile, token tile) items, and the ring runs on from one item
 //     into the next.  Rows per warp, slices and rows per item follow a cost model
 //     (see plan): few rows are split along K, many are dealt out evenly.
-// Measured on B200, L2 flushed: 65536 x 7168 (235 MB) with one token 55 us = 4.3 TB/s,
-// with eight 58 us, with thirteen 85-91 us; the copies alone take 43-46 us (55-61 with
-// thirteen).  ncu with one: 20 instructions a word in all, 60 % of the issue slots; with
-// thirteen 25 and 53 %, most stalls on results of the instructions before: bound by
-// the latency and issue of the unpacking.
+// Measured on B200, one call after another: 65536 x 7168 (235 MB), groups of 128, bf16, with
+// one token 51 us = 4.6 TB/s, with eight 53, with thirteen 78; groups of 64 with zero
+// points, fp16, thirteen 85.  With parts left out (one / thirteen tokens, groups of 128):
+// copies alone 44 / 51, without the products 44 / 54, without the unpacking 47 / 68.  So
+// neither part alone adds much to the copies: a warp's products wait for its unpacking and
+// its sums for the products, two warps a scheduler (four with eight tokens) do not hide it
+// all, and 46 % (61 %) of the issue slots are taken, 20 (17) instructions a word.
 // The warp MMA, not tcgen05: a form that unpacks into tensor memory (the codes as A,
 // 128 rows x 64 k a step, sixteen warps) was built and gave 88-94 us for one token and
 // 94-106 for thirteen.  Its products cost next to nothing (9 cycles for 128 x 16 x 16),
@@ -646,8 +648,11 @@ static double rounds(double items, int at_once, bool about) {
 // Items need not be full: N = 65536 makes 256 items of 256 rows, two on 108 SMs and
 // one on 40, but 293 of 224 rows, two on nearly all (58 -> 55 us with one token).  A
 // warp's last rows cost about half as much as the mean (its other rows hide them).
-// Over 59 calls the plan was 1.7 % slower than the best of all plans (mean; 20 % at most).
-static Plan plan(int NT, double tiles, bool about, int N, int K, int G, int sms) {
+// The width of a group and zero points are not in it (47 tokens x 6 of 64 experts,
+// 7168 x 2048, groups of 32 with zero points: 102 us by the model, 126-143 measured); what
+// counts is the order of the plans.  Over 59 calls of all widths the plan was 3 % slower
+// than the best of all plans (mean; 23 % at most).
+static Plan plan(int NT, double tiles, bool about, int N, int K, int sms) {
   Plan best = {2, kWarps, 2, 1e30};
   const int KB = (K + kBlkK - 1) / kBlkK;
   for (int R = 2; R <= 4; R += 2) {
@@ -764,7 +769,7 @@ static void choose(Args& a, bool experts, int tokens, int sms, int* NT, int* R) 
       tile[i] = static_cast<int>((a.rows + n - 1) / n);      // evenly filled
       tiles = static_cast<double>(n);
     }
-    p[i] = plan(i + 1, tiles, experts && tokens > 1, a.N, a.K, a.G, sms);
+    p[i] = plan(i + 1, tiles, experts && tokens > 1, a.N, a.K, sms);
   }
   const int i = tile[1] > 8 && p[1].us < p[0].us;
   *NT = i + 1;

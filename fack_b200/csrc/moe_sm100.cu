@@ -18,12 +18,12 @@
 // crosses HBM once and no sum needs an atomic.  Every index read from a plan
 // is range-checked before it is used as an address.
 //
-// Measured on B200 (graph replay, share of the 6464 GB/s copy): gather 8192 x 8 rows
-// of 7168 bf16 176 us (0.93, in L2's favour at smaller sizes), 4096 x 6 of 4096 fp16
-// 39 (0.92); combine 154 and 39 (0.93); combine's gradients 4096 x 6 x 4096 74 (0.92);
-// the quantising gather 4095 x 4 of 7168 fp32 40 (0.93), 8192 x 2 of 7168 bf16 57
-// (0.65: a division and a conversion an element cost more than two bytes in and two
-// out).  Few tokens are bound by latency: 2-4 us to 16 tokens.
+// Measured on B200 (calls one after another in a replayed graph, share of the 6464 GB/s
+// copy): gather 8192 x 8 rows of 7168 bf16 180 us (0.91), 4096 x 6 of 4096 fp16 39.5
+// (0.92); combine 155 (1.05) and 39.4 (0.92); combine's gradients 316 (0.98) and 74 (0.91);
+// the quantising gather 4095 x 4 of 7168 fp32 39.5 (0.93), 8192 x 2 of 7168 bf16 58 (0.64:
+// 25 instructions an element for two bytes in and two out fill 76 % of the issue slots).
+// Few tokens are bound by latency: 2.6-3.3 us to 16 tokens.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -110,8 +110,8 @@ __global__ void __launch_bounds__(1024) sort_count_kernel(const I* __restrict__ 
 // against 7.9 us for 4096 pairs over 256 experts), their rank is the warp's running
 // count plus the lanes before them, so order is kept without an atomic.  A column
 // scan over the warps then turns counts into rows.  With one block (hist NULL) the
-// counts of the first and only chunk are the histogram.  Bound by latency: 2.4 us
-// for one token's pairs, 11 us for 524288 over 64 experts in two launches.
+// counts of the first and only chunk are the histogram.  Bound by latency: 3.1 us
+// for one token's pairs, 9.5 us for 524288 over 64 experts in two launches.
 template <typename I>
 __global__ void __launch_bounds__(1024) sort_place_kernel(const I* __restrict__ ids, int64_t pairs, int64_t share, int E,
                                                           const int* __restrict__ hist, int* __restrict__ row_of,
@@ -324,9 +324,9 @@ __global__ void __launch_bounds__(256) gather_kernel(const void* __restrict__ xp
 }
 
 // out[t] = sum_j w[t, j] * y[row_of[t, j]] (w NULL: 1), fp32, slots in order.  A
-// thread has SL slots of U places of the row in flight, eight 16-byte loads
-// whether a token has two experts or eight: with two loads the rows of 16384 x 2
-// experts, 1024 wide bf16, came at 0.60 of the copy rate.
+// thread has SL slots of U places of the row in flight: two of two, four of two or eight
+// of one, four to eight 16-byte loads.  With one place the rows of 16384 x 2 experts,
+// 1024 wide bf16, came at 0.60 of the copy rate (two loads); with two it is 0.89, 17.5 us.
 template <typename T, int V, int SL, int U>
 __global__ void __launch_bounds__(256) combine_kernel(const T* __restrict__ y, int64_t ldy, const float* __restrict__ w,
                                                       int nvec, int topk, int64_t rows, const int* __restrict__ row_of,
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const T* __restrict__ y, i
 // (either may be NULL), one block a token.  The dot products are fp32: each
 // thread's own columns in order, then the lanes, then the warps.  Four slots at a
 // time (two places of the row when a token has two): with eight the registers leave
-// two blocks an SM and 4096 x 6 x 4096 took 122 instead of 103 us, launch included.
+// two blocks an SM and 4096 x 6 x 4096 fp16 takes 85 instead of 74 us.
 // dout's load waits for no index.
 template <typename T, int V, int SL, int U>
 __global__ void __launch_bounds__(256, 3) combine_bwd_kernel(const T* __restrict__ dout, int64_t ldd,

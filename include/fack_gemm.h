@@ -469,8 +469,9 @@ int fack_gemm_tn(int kind, const void* a, int64_t lda, const void* b, int b_pack
  * row) and run on FACK_DTYPE_F32, _BF16 or _F16 rows of D elements,
  * 1 <= D <= 2^20, in any alignment of the element type; rows that allow 16-byte
  * accesses (base, stride and D) go faster.  Sorted buffers hold T*topk rows; rows
- * without a pair are written as zeros (their scales as 1).  No output may overlap
- * an input or have rows that overlap.
+ * without a pair, those behind offsets[E], are written as zeros (their scales as
+ * 1); a row in front of it that no entry of row_of names (no plan of fack_moe_sort
+ * has one) is left as it is.  No output may overlap an input or have rows that overlap.
  *
  *   fack_moe_gather        y[row_of[t, j]] = x[t]
  *   fack_moe_gather_quant  xq, x_scale of row row_of[t, j] = the e4m3 codes and
