@@ -183,7 +183,7 @@ def _combine(y, weights, plan):
 
 def moe_gather_backward(dy: torch.Tensor, plan: MoePlan) -> torch.Tensor:
     """dx [T, D] of :func:`moe_gather` from dy [T*k, D]: each token's rows
-    summed in fp32, slots in order, rounded once."""
+    summed in fp32, slots in order, rounded once.  Not recorded by autograd."""
     _check_sorted(dy, plan)
     return _sum_rows(dy, None, plan.row_of)
 
@@ -206,7 +206,8 @@ def moe_combine_backward(dout: torch.Tensor, y: Optional[torch.Tensor], weights:
                          need_dy: bool = True, need_dweights: bool = True):
     """(dy [T*k, D], dweights fp32 [T, k]) of :func:`moe_combine` from dout
     [T, D]; None in the place of one that is not needed (``y`` may be None
-    without ``need_dweights``).  Rows of dy without a pair are zero."""
+    without ``need_dweights``).  Rows of dy without a pair are zero.  Not recorded
+    by autograd."""
     _check_rows(dout, "dout")
     dev = dout.device
     T, topk, _ = _check_plan(plan, dev)

@@ -522,7 +522,8 @@ int fack_moe_combine_bwd(const void* dout, int dtype, int64_t ldd, const void* y
  * w, scales and zeros are contiguous and 16-byte aligned.  N % 16 == 0;
  * G = 32, 64 or a multiple of 128; K % G == 0, K <= 2^20; M >= 1 (meant for M
  * up to about 32: more tokens are taken 8 or 16 at a time).  Products are exact, sums
- * fp32, one rounding to y's type; the same call gives the same bits.
+ * fp32 (those of up to 128 k before their scale is applied, so x times codes has
+ * to stay in its range), one rounding to y's type; the same call gives the same bits.
  * Capturable; allocates nothing.  y may not overlap an operand.
  *
  * fack_gemv_w4_experts: y [T*topk, N] from the weights of each sorted row's
